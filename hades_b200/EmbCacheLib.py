@@ -1025,3 +1025,48 @@ def cudaMergeSortedSlabs(ids, rows, cnt, seg_counts, seg_cap: int, mean: bool = 
                                              int(mean), uniq.data_ptr(), out.data_ptr(), counts.data_ptr(),
                                              num.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_ptr()))
     return uniq, out, counts, num
+
+
+# ---------------------------------------------------------------------------------------
+# token embeddings of language models (no counterpart in the reference)
+# ---------------------------------------------------------------------------------------
+def cudaEmbedding(weight, ids, scale: float = 1.0, padding_idx: int | None = None, dropout: float = 0.0, seed: int = 0,
+                  offset: int = 0, rng: torch.Tensor | None = None, dtype: torch.dtype | None = None, out=None):
+    """Rows of a table by token, [*ids.shape, dim]: scale * weight[ids] with a share ``dropout`` of the values dropped,
+    in one launch.  weight: [rows, dim] fp32, fp16 or bf16 on the GPU (or in pinned host memory), its rows at any even
+    distance; ids: int32 or int64 of any shape; dtype: of the result (that of weight); out: a result to write into.
+    Positions of ``padding_idx`` (any number, -1 too) give zeros; so do ids outside of the table, which also set
+    HB_ERR_INVALID in ``_lib.device_status()``.
+
+    The mask is that of ``cudaDropout`` over rows in the order of the ids.  seed, offset: which mask (``hb_drop_t``); the
+    gradient is found by the same two numbers.  rng: int64[2] on the GPU with both, read when the kernel runs."""
+    return (_lib._NATIVE or _lib.native()).embedding(weight, ids, scale, padding_idx, dropout, seed, offset, rng, dtype, out)
+
+
+def cudaEmbeddingGrad(ids, grad, num_embeddings: int, scale: float = 1.0, padding_idx: int | None = None,
+                      dropout: float = 0.0, seed: int = 0, offset: int = 0, rng: torch.Tensor | None = None,
+                      dtype: torch.dtype | None = None, out=None, accumulate: bool = False):
+    """Gradient of the table of ``cudaEmbedding`` from that of its result, [num_embeddings, dim] in dtype (that of grad):
+    tokens sorted once, every row of grad read once, sums in fp32 and in the same order every time.  accumulate: added to
+    ``out`` (rows of tokens that do not occur are not touched); else all rows of ``out`` are written."""
+    return (_lib._NATIVE or _lib.native()).embedding_grad(ids, grad, num_embeddings, scale, padding_idx, dropout, seed, offset,
+                                                          rng, dtype, out, accumulate)
+
+
+def cudaEmbeddingGradRows(ids, grad, num_embeddings: int, scale: float = 1.0, padding_idx: int | None = None,
+                          dropout: float = 0.0, seed: int = 0, offset: int = 0, rng: torch.Tensor | None = None,
+                          sync: bool = True):
+    """The gradient of ``cudaEmbeddingGrad`` as (distinct tokens ascending, their fp32 rows), cut to their number, which is
+    read on the host while the rows are added up.  sync=False: (tokens, rows, number on the device) at full size, for
+    ``SparseAdam.update(tokens, rows, is_unique=True, n_dev=number)``, and in captured graphs."""
+    return (_lib._NATIVE or _lib.native()).embedding_grad_rows(ids, grad, num_embeddings, scale, padding_idx, dropout, seed,
+                                                               offset, rng, sync)
+
+
+def cudaDropout(x, p: float, seed: int = 0, offset: int = 0, rng: torch.Tensor | None = None, scale: float = 1.0,
+                dtype: torch.dtype | None = None, out=None):
+    """scale * x with a share p of the values (in steps of 1/65536) set to zero and the others divided by the share kept,
+    the mask drawn from (seed, offset) and the value's (row, column) by a counter-based generator and never stored.  x:
+    fp32, fp16 or bf16, [..., dim], rows counted over the leading dimensions.  out may be x.  The gradient of the result
+    with respect to x is the same call on the gradient."""
+    return (_lib._NATIVE or _lib.native()).dropout(x, scale, p, seed, offset, rng, dtype, out)

@@ -136,6 +136,13 @@ PROTOTYPES: dict[str, tuple] = {
     "hb_step_join": (_int, [_p, _p]),
     "hb_step_backward": (_int, [_p, _p, _p, _i64, _p, _p, _p, _sz, _p]),
     "hb_fetch_serve": (_int, [_p, _p, _p, _p, _p, _i64, _p]),
+    "hb_embedding": (_int, [_p, _int, _i64, _i64, _i64, _p, _int, _i64, _i64, C.c_double, _p, _p, _int, _i64, _p]),
+    "hb_dropout": (_int, [_p, _int, _i64, _i64, _i64, C.c_double, _p, _p, _int, _i64, _p]),
+    "hb_embedding_grad_workspace_bytes": (_sz, [_i64, _i64]),
+    "hb_embedding_grad": (_int, [_p, _int, _i64, _i64, _p, _int, _i64, _i64, C.c_double, _p, _i64, _p, _int, _i64, _int,
+                                 _p, _sz, _p]),
+    "hb_embedding_grad_rows": (_int, [_p, _int, _i64, _i64, _p, _int, _i64, _i64, C.c_double, _p, _i64, _p, _p, _p, _p,
+                                      _sz, _p]),
 }
 
 
@@ -157,6 +164,11 @@ class OptimDesc(C.Structure):
     _fields_ = [("kind", _int), ("emb_elem_bytes", _int), ("emb", _p), ("s0", _p), ("s1", _p), ("step", _p),
                 ("id_offset", _i64), ("id_stride", _i64), ("rows", _i64), ("lr", C.c_double), ("beta1", C.c_double),
                 ("beta2", C.c_double), ("eps", C.c_double)]
+
+
+class DropDesc(C.Structure):
+    """hb_drop_t"""
+    _fields_ = [("p", C.c_double), ("seed", C.c_uint64), ("offset", C.c_uint64), ("rng", _p)]
 
 
 class StagingDesc(C.Structure):

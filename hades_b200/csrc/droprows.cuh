@@ -1,0 +1,221 @@
+// Rows of fp32, fp16 or bf16 values in blocks of eight columns, and the dropout of such rows: what the embedding lookup,
+// its gradient and the dropout of rows that exist already share.
+//
+// Dropout: value (row, column) is kept where the 16 bits that the generator gives its place are at least T; T of 65536
+// values are dropped, and what is kept is multiplied by 65536 / (65536 - T).  The generator is Philox4x32 with ten rounds
+// (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011): counter (column / 8, row, offset's
+// low and high word), key the seed.  A call's 128 bits are the draws of eight neighbouring columns, so that a place needs
+// no state and no mask in memory, forward and backward passes agree whatever kernel or layout they use, and the ten rounds
+// (some 60 instructions) cost a value 8; with 32 bits a value they would cost 15, which is more than the memory that a
+// bf16 value crosses takes.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cmath>
+#include <type_traits>
+
+#include "launch.cuh"
+
+namespace hb {
+
+constexpr int kBlockCols = 8;  // columns of a block: a thread's, and a call's of the generator
+
+struct Dropout {
+  uint32_t drop_below;  // T; 0: nothing is dropped
+  float factor;         // of what is kept: scale * 65536 / (65536 - T), rounded once
+  uint64_t seed, offset;
+  const int64_t* rng;   // nullable, device: seed and offset as they are when the kernel runs
+};
+
+// The checks and the numbers of a call's (scale, dropout); drop nullable.
+static inline int dropout_of(const char* who, double scale, const hb_drop_t* drop, Dropout* out) {
+  HB_CHECK_ARG(!drop || (drop->p >= 0.0 && drop->p <= 1.0), "%s: the dropout probability must be in [0, 1]", who);
+  const double t = drop ? std::floor(drop->p * 65536.0 + 0.5) : 0.0;
+  const double f = t < 65536.0 ? scale * 65536.0 / (65536.0 - t) : 0.0;
+  HB_CHECK_ARG(std::isfinite(scale) && std::isfinite((float)f), "%s: the scale must be finite", who);
+  out->drop_below = (uint32_t)t;
+  out->factor = (float)f;
+  out->seed = drop ? drop->seed : 0;
+  out->offset = drop ? drop->offset : 0;
+  out->rng = drop && t > 0.0 ? drop->rng : nullptr;
+  return HB_OK;
+}
+
+static inline int type_bytes(int type) { return type == HB_TYPE_F32 ? 4 : 2; }
+static inline bool type_known(int type) { return type == HB_TYPE_F32 || type == HB_TYPE_F16 || type == HB_TYPE_BF16; }
+
+// Whether matrices of rows of dim values share memory (as ranges of addresses).
+static inline bool overlap(const void* a, int64_t a_stride, int a_type, int64_t a_rows, const void* b, int64_t b_stride,
+                           int b_type, int64_t b_rows, int64_t dim) {
+  if (a_rows <= 0 || b_rows <= 0) return false;
+  const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
+  const uintptr_t a1 = a0 + (uintptr_t)(((a_rows - 1) * a_stride + dim) * type_bytes(a_type));
+  const uintptr_t b1 = b0 + (uintptr_t)(((b_rows - 1) * b_stride + dim) * type_bytes(b_type));
+  return a0 < b1 && b0 < a1;
+}
+
+// Bytes that a thread can move at once of every block of a matrix: as wide as its rows' starts allow, at most 16.
+static inline int access_bytes(const void* base, int64_t stride, int type) {
+  const uint64_t bits = (uint64_t)(uintptr_t)base | (uint64_t)(stride * type_bytes(type)) | 16u;
+  return (int)(bits & (~bits + 1));
+}
+
+#ifdef __CUDACC__
+
+struct PhiloxKey { uint32_t k0, k1, offset_lo, offset_hi; };
+
+__device__ __forceinline__ PhiloxKey philox_key(const Dropout& d) {
+  const uint64_t seed = d.rng ? (uint64_t)d.rng[0] : d.seed, offset = d.rng ? (uint64_t)d.rng[1] : d.offset;
+  return {(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)offset, (uint32_t)(offset >> 32)};
+}
+
+__device__ __forceinline__ uint4 philox(uint4 c, uint32_t k0, uint32_t k1) {
+#pragma unroll
+  for (int i = 0; i < 10; ++i) {
+    const uint64_t a = (uint64_t)c.x * 0xD2511F53u, b = (uint64_t)c.z * 0xCD9E8D57u;
+    c = make_uint4((uint32_t)(b >> 32) ^ c.y ^ k0, (uint32_t)b, (uint32_t)(a >> 32) ^ c.w ^ k1, (uint32_t)a);
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return c;
+}
+
+// Multiplies a block by the factor; zeros where values are dropped, whatever they were.
+__device__ __forceinline__ void drop_block(float (&x)[kBlockCols], const PhiloxKey& k, uint32_t drop_below, float factor,
+                                           uint32_t block, uint32_t row) {
+  const uint4 w = philox(make_uint4(block, row, k.offset_lo, k.offset_hi), k.k0, k.k1);
+  const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x[2 * j] = (word[j] & 0xffffu) >= drop_below ? x[2 * j] * factor : 0.0f;
+    x[2 * j + 1] = (word[j] >> 16) >= drop_below ? x[2 * j + 1] * factor : 0.0f;
+  }
+}
+
+// ---- a block in memory: eight values as the words that they take -------------------------------------------------------
+template <typename T> constexpr int block_words() { return kBlockCols * (int)sizeof(T) / 4; }
+
+template <int W> struct Words { uint32_t w[W]; };
+
+// Loads of what no other thread of the launch writes (an in-place call reads a value before it writes it, in one thread).
+// width: access_bytes of the matrix; cols: columns of the row from the block on, eight of a whole block.
+template <typename T>
+__device__ __forceinline__ void load_words(const T* p, int width, int cols, Words<block_words<T>()>& v) {
+  constexpr int W = block_words<T>();
+  if (cols < kBlockCols) {  // the end of a row
+#pragma unroll
+    for (int i = 0; i < W; ++i) v.w[i] = 0u;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        if (i < cols) v.w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kBlockCols; ++i)
+        if (i < cols) v.w[i / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
+    }
+  } else if (width == 16) {
+#pragma unroll
+    for (int i = 0; i < W; i += 4) {
+      const uint4 t = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i);
+      v.w[i] = t.x; v.w[i + 1] = t.y; v.w[i + 2] = t.z; v.w[i + 3] = t.w;
+    }
+  } else if (width == 8) {
+#pragma unroll
+    for (int i = 0; i < W; i += 2) {
+      const uint2 t = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint32_t*>(p) + i);
+      v.w[i] = t.x; v.w[i + 1] = t.y;
+    }
+  } else if (width == 4) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) v.w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+  } else {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < W; ++i) v.w[i] = (uint32_t)h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_words(T* p, int width, int cols, const Words<block_words<T>()>& v) {
+  constexpr int W = block_words<T>();
+  if (cols < kBlockCols) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        if (i < cols) reinterpret_cast<uint32_t*>(p)[i] = v.w[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kBlockCols; ++i)
+        if (i < cols) reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(v.w[i / 2] >> (16 * (i & 1)));
+    }
+  } else if (width == 16) {
+#pragma unroll
+    for (int i = 0; i < W; i += 4)
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(p) + i) = make_uint4(v.w[i], v.w[i + 1], v.w[i + 2], v.w[i + 3]);
+  } else if (width == 8) {
+#pragma unroll
+    for (int i = 0; i < W; i += 2)
+      *reinterpret_cast<uint2*>(reinterpret_cast<uint32_t*>(p) + i) = make_uint2(v.w[i], v.w[i + 1]);
+  } else if (width == 4) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) reinterpret_cast<uint32_t*>(p)[i] = v.w[i];
+  } else {
+    uint16_t* h = reinterpret_cast<uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      h[2 * i] = (uint16_t)v.w[i];
+      h[2 * i + 1] = (uint16_t)(v.w[i] >> 16);
+    }
+  }
+}
+
+// ---- words and values: everything between a load and a store is fp32, and rounded once ----------------------------------
+template <typename T>
+__device__ __forceinline__ void values_of(const Words<block_words<T>()>& v, float (&x)[kBlockCols]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(v.w[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float2 f;
+      if constexpr (std::is_same_v<T, __half>) f = __half22float2(*reinterpret_cast<const __half2*>(&v.w[i]));
+      else f = make_float2(__uint_as_float(v.w[i] << 16), __uint_as_float(v.w[i] & 0xffff0000u));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void words_of(const float (&x)[kBlockCols], Words<block_words<T>()>& v) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v.w[i] = __float_as_uint(x[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        v.w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        v.w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+  }
+}
+
+#endif  // __CUDACC__
+
+// f(T{}) for the value type of a matrix
+template <typename F>
+int with_type(int type, F f) {
+  if (type == HB_TYPE_F32) return f(float{});
+  if (type == HB_TYPE_F16) return f(__half{});
+  return f(__nv_bfloat16{});
+}
+
+}  // namespace hb

@@ -10,6 +10,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <atomic>
@@ -429,6 +430,210 @@ PyObject* step_backward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   });
 }
 
+// ---- token embeddings ---------------------------------------------------------------------------------------------------
+int value_type(at::ScalarType t, const char* what) {
+  if (t == at::kFloat) return HB_TYPE_F32;
+  if (t == at::kHalf) return HB_TYPE_F16;
+  if (t == at::kBFloat16) return HB_TYPE_BF16;
+  PyErr_Format(PyExc_RuntimeError, "Check failed: %s is fp32, fp16 or bf16", what);
+  throw Status();
+}
+at::ScalarType type_or(PyObject* o, at::ScalarType other) {
+  if (none(o)) return other;
+  if (!THPDtype_Check(o)) {
+    PyErr_SetString(PyExc_TypeError, "dtype: a torch.dtype is expected");
+    throw Status();
+  }
+  return reinterpret_cast<THPDtype*>(o)->scalar_type;
+}
+double number(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw Status();
+  return v;
+}
+uint64_t word64(PyObject* o) {  // OverflowError outside of [0, 2^64)
+  const unsigned long long v = PyLong_AsUnsignedLongLong(o);
+  if (v == (unsigned long long)-1 && PyErr_Occurred()) throw Status();
+  return v;
+}
+// p, seed, offset, rng | None
+hb_drop_t drop_of(PyObject* const* a, const at::Device& dev) {
+  hb_drop_t d{number(a[0]), word64(a[1]), word64(a[2]), nullptr};
+  if (!none(a[3])) {
+    const at::Tensor& rng = tensor(a[3], "rng");
+    require(rng.device() == dev && rng.scalar_type() == at::kLong && rng.numel() == 2 && rng.is_contiguous(),
+            "rng is an int64 tensor of two (seed, offset) on the device of the call");
+    d.rng = rng.data_ptr<int64_t>();
+  }
+  return d;
+}
+// [rows, dim] of a tensor whose last dimension is dim: the distance of its rows, or -1 where they are not evenly spaced.
+int64_t row_stride(const at::Tensor& t) {
+  const int64_t k = t.dim();
+  if (k == 0 || (t.size(k - 1) > 1 && t.stride(k - 1) != 1)) return -1;
+  int64_t stride = 0, rows = 1;  // rows of the inner dimensions so far
+  for (int64_t d = k - 2; d >= 0; --d) {
+    if (t.size(d) == 1) continue;
+    if (rows == 1) stride = t.stride(d);
+    else if (t.stride(d) != stride * rows) return -1;
+    rows *= t.size(d);
+  }
+  return rows == 1 ? t.size(k - 1) : stride;
+}
+// A matrix to read: itself, or a contiguous copy where its rows are not evenly spaced.
+at::Tensor readable(const at::Tensor& t, int64_t& stride) {
+  stride = row_stride(t);
+  if (stride >= 0) return t;
+  stride = t.size(t.dim() - 1);
+  return t.contiguous();
+}
+at::Tensor token_ids(const at::Tensor& t, const at::Device& dev) {
+  require(t.is_cuda() && t.device() == dev, "ids lie on the device of the rows");
+  if (t.scalar_type() != at::kLong && t.scalar_type() != at::kInt) {
+    PyErr_SetString(PyExc_RuntimeError, "ID can only be int32 or int64");
+    throw Status();
+  }
+  return t.contiguous();
+}
+int64_t padding_of(PyObject* o) { return none(o) ? HB_NO_PADDING : integer(o); }
+
+// An output that the caller gives: its shape, where its rows are.
+at::Tensor given_output(PyObject* o, at::IntArrayRef size, const at::Device& dev, int64_t& stride) {
+  const at::Tensor& t = tensor(o, "out");
+  require(t.device() == dev && t.sizes() == size, "out has the shape of the result and lies on its device");
+  stride = row_stride(t);
+  require(stride >= 0, "the rows of out are contiguous and evenly spaced");
+  return t;
+}
+
+// embedding(weight, ids, scale, padding | None, p, seed, offset, rng | None, dtype | None, out | None)
+PyObject* embedding(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    arity(n_args, 10, "embedding");
+    const at::Tensor &weight = tensor(a[0], "weight"), &given = tensor(a[1], "ids");
+    require(given.is_cuda(), "ids is a CUDA tensor");
+    const at::Device dev = given.device();
+    require(weight.dim() == 2 && weight.size(1) > 0, "weight is [rows, dim]");
+    require(weight.is_cuda() ? weight.device() == dev : weight.is_pinned(),
+            "weight lies on the device of the ids, or in pinned host memory");
+    require(weight.size(1) == 1 || weight.stride(1) == 1, "the rows of weight are contiguous");
+    const int wt = value_type(weight.scalar_type(), "weight");
+    const at::ScalarType type = none(a[9]) ? type_or(a[8], weight.scalar_type()) : tensor(a[9], "out").scalar_type();
+    require(none(a[9]) || none(a[8]) || type_or(a[8], type) == type, "out.dtype == dtype");
+    const int ot = value_type(type, "out");
+    c10::cuda::CUDAGuard guard(dev);
+    const at::Tensor ids = token_ids(given, dev);
+    const hb_drop_t drop = drop_of(a + 4, dev);
+    const int64_t n = ids.numel(), dim = weight.size(1);
+    c10::SmallVector<int64_t, 5> size(given.sizes().begin(), given.sizes().end());
+    size.push_back(dim);
+    int64_t stride = dim;
+    at::Tensor out = none(a[9]) ? cuda_empty(size, type, dev) : given_output(a[9], size, dev, stride);
+    check(hb_embedding(weight.data_ptr(), wt, weight.stride(0), weight.size(0), dim, ids.data_ptr(), (int)ids.element_size(),
+                       n, padding_of(a[3]), number(a[2]), &drop, out.data_ptr(), ot, stride, stream_of(dev)));
+    return THPVariable_Wrap(out);
+  });
+}
+
+// dropout(x, scale, p, seed, offset, rng | None, dtype | None, out | None)
+PyObject* dropout(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    arity(n_args, 8, "dropout");
+    const at::Tensor& given = tensor(a[0], "x");
+    require(given.is_cuda() && given.dim() >= 1 && given.size(given.dim() - 1) > 0, "x is a CUDA tensor [..., dim]");
+    const at::Device dev = given.device();
+    const int xt = value_type(given.scalar_type(), "x");
+    const at::ScalarType type = none(a[7]) ? type_or(a[6], given.scalar_type()) : tensor(a[7], "out").scalar_type();
+    require(none(a[7]) || none(a[6]) || type_or(a[6], type) == type, "out.dtype == dtype");
+    const int ot = value_type(type, "out");
+    c10::cuda::CUDAGuard guard(dev);
+    int64_t x_stride = 0;
+    const at::Tensor x = readable(given, x_stride);
+    const hb_drop_t drop = drop_of(a + 2, dev);
+    const int64_t dim = x.size(x.dim() - 1);
+    int64_t stride = dim;
+    at::Tensor out = none(a[7]) ? cuda_empty(x.sizes(), type, dev) : given_output(a[7], x.sizes(), dev, stride);
+    check(hb_dropout(x.data_ptr(), xt, x_stride, x.numel() / dim, dim, number(a[1]), &drop, out.data_ptr(), ot, stride,
+                     stream_of(dev)));
+    return THPVariable_Wrap(out);
+  });
+}
+
+// What both forms of the gradient take: ids, grads, num_rows
+struct GradInputs {
+  at::Device dev;
+  at::Tensor ids, grads;
+  int type;
+  int64_t n, dim, stride = 0, rows;
+  GradInputs(PyObject* const* a) : dev(at::kCPU) {
+    const at::Tensor &t = tensor(a[0], "ids"), &g = tensor(a[1], "grad");
+    require(g.is_cuda() && g.dim() >= 1 && g.size(g.dim() - 1) > 0, "grad is a CUDA tensor [..., dim]");
+    dev = g.device();
+    type = value_type(g.scalar_type(), "grad");
+    dim = g.size(g.dim() - 1);
+    require(g.numel() / dim == t.numel(), "grad has a row for every id");
+    rows = integer(a[2]);
+    require(rows >= 0, "num_embeddings >= 0");
+    c10::cuda::CUDAGuard guard(dev);
+    ids = token_ids(t, dev);
+    grads = readable(g, stride);
+    n = ids.numel();
+  }
+};
+
+// embedding_grad(ids, grads, num_rows, scale, padding | None, p, seed, offset, rng | None, dtype | None, out | None, accumulate)
+PyObject* embedding_grad(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    arity(n_args, 12, "embedding_grad");
+    const GradInputs in(a);
+    const bool accumulate = PyObject_IsTrue(a[11]);
+    require(!accumulate || !none(a[10]), "accumulate adds to a given out");
+    const at::ScalarType type = none(a[10]) ? type_or(a[9], in.grads.scalar_type()) : tensor(a[10], "out").scalar_type();
+    require(none(a[10]) || none(a[9]) || type_or(a[9], type) == type, "out.dtype == dtype");
+    const int ot = value_type(type, "out");
+    c10::cuda::CUDAGuard guard(in.dev);
+    const hb_drop_t drop = drop_of(a + 5, in.dev);
+    int64_t stride = in.dim;
+    at::Tensor out = none(a[10]) ? cuda_empty({in.rows, in.dim}, type, in.dev)
+                                 : given_output(a[10], {in.rows, in.dim}, in.dev, stride);
+    const size_t need = hb_embedding_grad_workspace_bytes(in.n, in.dim);
+    const at::Tensor ws = cuda_empty({(int64_t)need}, at::kByte, in.dev);
+    check(hb_embedding_grad(in.ids.data_ptr(), (int)in.ids.element_size(), in.n, padding_of(a[4]), in.grads.data_ptr(), in.type,
+                            in.stride, in.dim, number(a[3]), &drop, in.rows, out.data_ptr(), ot, stride, accumulate,
+                            ws.data_ptr(), need, stream_of(in.dev)));
+    return THPVariable_Wrap(out);
+  });
+}
+
+// embedding_grad_rows(ids, grads, num_rows, scale, padding | None, p, seed, offset, rng | None, sync) -> (tokens, rows), cut to
+// the number of distinct tokens, which is awaited while the rows are being added up; sync false: (tokens, rows, number)
+PyObject* embedding_grad_rows(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    arity(n_args, 10, "embedding_grad_rows");
+    const GradInputs in(a);
+    const bool sync = PyObject_IsTrue(a[9]);
+    c10::cuda::CUDAGuard guard(in.dev);
+    void* st = stream_of(in.dev);
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    if (sync && cudaStreamIsCapturing(static_cast<cudaStream_t>(st), &capturing) == cudaSuccess)
+      require(capturing == cudaStreamCaptureStatusNone, "sync=False in a captured graph (the number is not read on the host)");
+    const hb_drop_t drop = drop_of(a + 5, in.dev);
+    at::Tensor uniq = cuda_empty({in.n}, at::kLong, in.dev), rows = cuda_empty({in.n, in.dim}, at::kFloat, in.dev);
+    const size_t need = hb_embedding_grad_workspace_bytes(in.n, in.dim);
+    const at::Tensor ws = cuda_empty({(int64_t)need}, at::kByte, in.dev);
+    at::Tensor count;
+    if (!sync) count = cuda_empty({1}, at::kLong, in.dev);
+    if (sync && in.n == 0) return pack({THPVariable_Wrap(uniq), THPVariable_Wrap(rows)});
+    int64_t* num = sync ? t_word.arm() : count.data_ptr<int64_t>();
+    check(hb_embedding_grad_rows(in.ids.data_ptr(), (int)in.ids.element_size(), in.n, padding_of(a[4]), in.grads.data_ptr(),
+                                 in.type, in.stride, in.dim, number(a[3]), &drop, in.rows, uniq.data_ptr<int64_t>(),
+                                 rows.data_ptr<float>(), num, ws.data_ptr(), need, st));
+    if (!sync) return pack({THPVariable_Wrap(uniq), THPVariable_Wrap(rows), THPVariable_Wrap(count)});
+    const int64_t u = t_word.wait(static_cast<cudaStream_t>(st));
+    return pack({THPVariable_Wrap(uniq.narrow(0, 0, u)), THPVariable_Wrap(rows.narrow(0, 0, u))});
+  });
+}
+
 PyObject* set_error_class(PyObject*, PyObject* cls) {
   Py_XINCREF(cls);
   Py_XSETREF(g_error, cls);
@@ -445,6 +650,10 @@ PyMethodDef g_methods[] = {
     {"staging_flush", HB_FAST(staging_flush), nullptr},
     {"step_forward", HB_FAST(step_forward), nullptr},
     {"step_backward", HB_FAST(step_backward), nullptr},
+    {"embedding", HB_FAST(embedding), nullptr},
+    {"dropout", HB_FAST(dropout), nullptr},
+    {"embedding_grad", HB_FAST(embedding_grad), nullptr},
+    {"embedding_grad_rows", HB_FAST(embedding_grad_rows), nullptr},
     {"set_error_class", set_error_class, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

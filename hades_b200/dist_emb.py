@@ -24,6 +24,7 @@ import torch
 import torch.nn as nn
 
 from . import EmbCacheLib as E
+from . import token_emb
 from .pipeline import EmbeddingPath
 
 
@@ -82,15 +83,31 @@ class DistEmbeddingTensor:
 
 
 class DistEmb(nn.Module):
-    """``nn.Module`` face of the layer (dist_emb.py:11-51)."""
+    """``nn.Module`` face of the layer (dist_emb.py:11-51).  scale, dropout (not in the reference): what it returns is
+    scale times the rows, in training with a share ``dropout`` of the values dropped (``token_emb.dropout``, seeded by
+    ``seed``); gradients reach the rows through both."""
 
-    def __init__(self, path: EmbeddingPath, name: str = "emb_layer"):
+    def __init__(self, path: EmbeddingPath, name: str = "emb_layer", scale: float = 1.0, dropout: float = 0.0,
+                 seed: int | None = None):
         super().__init__()
+        E._check(0.0 <= dropout <= 1.0, "0 <= dropout <= 1")
         self.emb_dim = path.dim
         self.sparse_emb = DistEmbeddingTensor(path, name)
+        self.scale, self.dropout = float(scale), float(dropout)
+        self.seeds = token_emb.DropoutSeeds(seed) if dropout else None
 
     def forward(self, idx: torch.Tensor) -> torch.Tensor:
-        return self.sparse_emb(idx, None, self.training)
+        if self.training:
+            rows = self.sparse_emb(idx, None, True)
+            if self.dropout:
+                return token_emb.dropout(rows, self.dropout, scale=self.scale, **self.seeds.next())
+            return rows if self.scale == 1.0 else token_emb.dropout(rows, 0.0, scale=self.scale)
+        path = self.sparse_emb.path
+        if self.scale == 1.0:
+            return self.sparse_emb(idx, None, False)
+        if path.shared is None:
+            return E.cudaEmbedding(path.table, idx.to(path.device, non_blocking=True), self.scale)
+        return E.cudaDropout(self.sparse_emb(idx, None, False), 0.0, scale=self.scale)
 
 
 class DistembSparseGradOptimizer:

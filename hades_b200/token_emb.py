@@ -1,0 +1,145 @@
+"""Token embeddings of language models with autograd: scaled lookup, dropout whose mask is not stored, gradients by
+sorted tokens (``cudaEmbedding``, ``cudaDropout``, ``cudaEmbeddingGrad`` of ``EmbCacheLib``).  The reference has no such
+layer; ``dist_emb.DistEmb`` takes its dropout from here.
+
+    layer = TokenEmbedding(50_000, 1_024, scale=32.0, padding_idx=0, dropout=0.1, dtype=torch.bfloat16)
+    h = layer(tokens)                 # [*tokens.shape, 1024]
+    loss(h).backward()                # layer.weight.grad: every row, in the type of the weights
+
+With a sparse optimiser the table is a ``ShardedEmbedding`` and the looked-up rows are the leaf, as in ``DistEmb``:
+
+    h = cudaEmbedding(emb.weight, tokens, scale=s).requires_grad_()
+    loss(h).backward()
+    rows = cudaEmbeddingGradRows(tokens, h.grad, emb.num_embeddings, scale=s, sync=False)
+    optimizer.update(rows[0], rows[1], is_unique=True, n_dev=rows[2])
+
+Captured graphs: masks come from numbers that a graph would repeat at every replay, so that a captured layer keeps them on
+the GPU (``seed_on_device=True``).  A graph of the same weights that was built outside of the capture must be gone before:
+its gradient accumulation belongs to another stream, which a capture cannot wait for, so both calls below refuse it.
+"""
+from __future__ import annotations
+
+import weakref
+
+import torch
+import torch.nn as nn
+from torch.utils.weak import WeakIdKeyDictionary
+
+from . import EmbCacheLib as E
+
+_GRAPHS = WeakIdKeyDictionary()  # leaf -> the live graphs of it that were built outside of a capture
+
+
+def _capturing() -> bool:
+    return torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+
+
+def _note(ctx, leaf: torch.Tensor) -> None:
+    """Remember on a leaf which graphs of it live that were built outside of a capture; inside of one there may be none."""
+    ctx.captured = _capturing()
+    if not (leaf.requires_grad and leaf.is_leaf):
+        return
+    graphs = _GRAPHS.get(leaf)
+    if ctx.captured:
+        if graphs:
+            raise RuntimeError("Check failed: a graph of the same leaf that was built outside of this capture still lives "
+                               "(drop its outputs first)")
+        return
+    if graphs is None:
+        graphs = _GRAPHS[leaf] = weakref.WeakSet()
+    graphs.add(ctx)
+
+
+def _refuse_foreign(ctx) -> None:
+    if _capturing() and not ctx.captured:
+        raise RuntimeError("Check failed: the forward pass belongs to the capture that its backward pass is in")
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, ids, scale, padding_idx, dropout, seed, offset, rng, dtype):
+        _note(ctx, weight)
+        ctx.save_for_backward(ids, rng)
+        ctx.call = (weight.size(0), scale, padding_idx, dropout, seed, offset, weight.dtype)
+        return E.cudaEmbedding(weight, ids, scale, padding_idx, dropout, seed, offset, rng, dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        _refuse_foreign(ctx)
+        ids, rng = ctx.saved_tensors
+        rows, scale, padding_idx, dropout, seed, offset, dtype = ctx.call
+        return (E.cudaEmbeddingGrad(ids, grad, rows, scale, padding_idx, dropout, seed, offset, rng, dtype),
+                None, None, None, None, None, None, None, None)
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, seed, offset, rng, scale, dtype):
+        _note(ctx, x)
+        ctx.save_for_backward(rng)
+        ctx.call = (p, seed, offset, scale, x.dtype)
+        return E.cudaDropout(x, p, seed, offset, rng, scale, dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        _refuse_foreign(ctx)
+        (rng,) = ctx.saved_tensors
+        p, seed, offset, scale, dtype = ctx.call
+        return E.cudaDropout(grad, p, seed, offset, rng, scale, dtype), None, None, None, None, None, None
+
+
+def embedding(weight, ids, scale: float = 1.0, padding_idx: int | None = None, dropout: float = 0.0, seed: int = 0,
+              offset: int = 0, rng: torch.Tensor | None = None, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``cudaEmbedding``, differentiable in weight (all of whose rows the gradient has, zeros where no token points)."""
+    return _Embedding.apply(weight, ids, scale, padding_idx, dropout, seed, offset, rng, dtype)
+
+
+def dropout(x, p: float, seed: int = 0, offset: int = 0, rng: torch.Tensor | None = None, scale: float = 1.0,
+            dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``cudaDropout``, differentiable in x."""
+    return _Dropout.apply(x, p, seed, offset, rng, scale, dtype)
+
+
+class DropoutSeeds:
+    """The (seed, offset) of a layer's masks: a seed, and the number of masks so far.  seed None: drawn from torch's
+    default generator.  on_device: both are kept on that GPU and advanced there, so that every replay of a captured graph
+    draws another mask."""
+
+    def __init__(self, seed: int | None = None, on_device=None):
+        self.seed = int(torch.randint(0, 1 << 62, (1,)).item()) if seed is None else int(seed)
+        E._check(0 <= self.seed < 1 << 63, "0 <= seed < 2^63")
+        self.offset = 0
+        self.state = None
+        if on_device is not None:
+            self.state = torch.tensor([self.seed, 0], dtype=torch.int64, device=on_device)
+
+    def next(self) -> dict:
+        """The next mask, as the arguments of ``cudaDropout`` and its like."""
+        if self.state is None:
+            self.offset += 1
+            return {"seed": self.seed, "offset": self.offset}
+        self.state[1] += 1
+        return {"rng": self.state.clone()}  # (the backward pass reads it after the next call has advanced the state)
+
+
+class TokenEmbedding(nn.Module):
+    """A table of [num_embeddings, embedding_dim] weights on the GPU, looked up by token.  Values are multiplied by
+    ``scale``; in training a share ``dropout`` of them is dropped."""
+
+    def __init__(self, num_embeddings: int, embedding_dim: int, scale: float = 1.0, padding_idx: int | None = None,
+                 dropout: float = 0.0, dtype=torch.float32, device="cuda", init_sigma: float = 0.02, seed: int | None = None,
+                 seed_on_device: bool = False):
+        super().__init__()
+        E._check(0.0 <= dropout <= 1.0, "0 <= dropout <= 1")
+        self.scale, self.padding_idx, self.dropout = float(scale), padding_idx, float(dropout)
+        weight = torch.empty((num_embeddings, embedding_dim), dtype=dtype, device=device).normal_(0.0, init_sigma)
+        if padding_idx is not None and 0 <= padding_idx < num_embeddings:
+            weight[padding_idx].zero_()
+        self.weight = nn.Parameter(weight)
+        self.seeds = DropoutSeeds(seed, device if seed_on_device else None)
+
+    def forward(self, ids: torch.Tensor) -> torch.Tensor:
+        drop = {"dropout": self.dropout, **self.seeds.next()} if self.training and self.dropout else {}
+        return embedding(self.weight, ids, self.scale, self.padding_idx, **drop)

@@ -787,6 +787,62 @@ int hb_step_join(hb_step_t* s, hb_stream_t stream);
 int hb_step_backward(hb_step_t* s, const hb_step_desc_t* d, const int64_t* ids, int64_t n, const float* grads,
                      int64_t* counters, void* workspace, size_t workspace_bytes, hb_stream_t stream);
 
+/* ------------------------------------------------------------------------- */
+/* Token embeddings of language models: scaled lookup, dropout, gradient by       */
+/* sorted tokens.  No counterpart in the reference (its layer ends at the fetched */
+/* rows, python/EmbCache/dist_emb.py:199-212).                                    */
+/* Values are fp32, fp16 or bf16, in any combination of input and output; they    */
+/* are computed in fp32 and rounded once.  Strides count values from one row to   */
+/* the next; the values of a row are contiguous.                                  */
+/* ------------------------------------------------------------------------- */
+#define HB_TYPE_F32 0
+#define HB_TYPE_F16 1
+#define HB_TYPE_BF16 2
+#define HB_NO_PADDING INT64_MIN
+
+/* Dropout whose mask is not stored.  T = floor(65536 p + 1/2) of 65536 values are dropped (so that p counts in steps of
+ * 1/65536) and the kept ones multiplied by 65536 / (65536 - T).  Value (row, column) is kept where its 16 bits are at
+ * least T: half column % 2 (the even column's is the low one) of word column % 8 / 2 of Philox4x32-10 with counter
+ * (column / 8, row, offset's low word, offset's high word) and the seed as its key.  Calls of one seed draw different
+ * masks by different offsets; the same (seed, offset) and shape give the same mask in every call below, which is how
+ * a backward pass finds it.  Dropped values are +0 whatever they were. */
+typedef struct hb_drop {
+  double p;           /* in [0, 1] */
+  uint64_t seed, offset;
+  const int64_t* rng; /* nullable, device int64[2]: seed and offset as they are when the kernel runs (captured graphs) */
+} hb_drop_t;
+
+/* out[i, :] = dropped(scale * weight[ids[i], :]), row i of the mask for position i.  A position whose id is padding_idx
+ * (HB_NO_PADDING: none) gives zeros; so does an id outside of [0, num_rows), which raises HB_ERR_INVALID in the device
+ * status word.  weight may be pinned host memory.  drop nullable. */
+int hb_embedding(const void* weight, int weight_type, int64_t weight_stride, int64_t num_rows, int64_t dim,
+                 const void* ids, int idx_bytes, int64_t n, int64_t padding_idx, double scale,
+                 const hb_drop_t* drop /* nullable, host */, void* out, int out_type, int64_t out_stride,
+                 hb_stream_t stream);
+
+/* y[i, :] = dropped(scale * x[i, :]); y may be x.  Its gradient is the same call on the gradient of y. */
+int hb_dropout(const void* x, int x_type, int64_t x_stride, int64_t n, int64_t dim, double scale,
+               const hb_drop_t* drop /* nullable, host */, void* y, int y_type, int64_t y_stride, hb_stream_t stream);
+
+/* Gradient of the table of hb_embedding from the gradients of its output: out[v, :] = scale * (sum over the positions i
+ * of token v of dropped(grads[i, :])), all num_rows rows, zeros where a token does not occur; accumulate: added to what out
+ * holds, rows of other tokens untouched.  Positions of padding_idx or of ids outside of the table (HB_ERR_INVALID in the
+ * status word) take no part.  Sums are in fp32, in an order that depends on n and dim alone.  workspace:
+ * hb_embedding_grad_workspace_bytes(n, dim), for hb_embedding_grad_rows too (0: sizes that are refused). */
+size_t hb_embedding_grad_workspace_bytes(int64_t n, int64_t dim);
+int hb_embedding_grad(const void* ids, int idx_bytes, int64_t n, int64_t padding_idx, const void* grads, int grad_type,
+                      int64_t grad_stride, int64_t dim, double scale, const hb_drop_t* drop /* nullable, host */,
+                      int64_t num_rows, void* out, int out_type, int64_t out_stride, int accumulate, void* workspace,
+                      size_t workspace_bytes, hb_stream_t stream);
+
+/* The same as distinct tokens, ascending, and their rows, for a sparse optimiser (hb_sparse_adam / hb_sparse_adagrad with
+ * n_dev = num_unique): uniq_ids and rows hold n entries, of which *num_unique (device) are written; the entries of
+ * uniq_ids behind them are undefined. */
+int hb_embedding_grad_rows(const void* ids, int idx_bytes, int64_t n, int64_t padding_idx, const void* grads,
+                           int grad_type, int64_t grad_stride, int64_t dim, double scale,
+                           const hb_drop_t* drop /* nullable, host */, int64_t num_rows, int64_t* uniq_ids, float* rows,
+                           int64_t* num_unique, void* workspace, size_t workspace_bytes, hb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
