@@ -56,13 +56,34 @@ static inline bool overlap(const void* a, int64_t a_stride, int a_type, int64_t 
   return a0 < b1 && b0 < a1;
 }
 
-// Bytes that a thread can move at once of every block of a matrix: as wide as its rows' starts allow, at most 16.
+// Bytes that a thread can move at once of every block of a matrix: as wide as its rows' starts allow, at most a block
+// (32 of fp32, 16 of the others).
 static inline int access_bytes(const void* base, int64_t stride, int type) {
-  const uint64_t bits = (uint64_t)(uintptr_t)base | (uint64_t)(stride * type_bytes(type)) | 16u;
+  const uint64_t bits = (uint64_t)(uintptr_t)base | (uint64_t)(stride * type_bytes(type)) | (uint64_t)(kBlockCols * type_bytes(type));
   return (int)(bits & (~bits + 1));
+}
+static inline bool whole_blocks(const void* base, int64_t stride, int type, int64_t dim) {
+  return dim % kBlockCols == 0 && access_bytes(base, stride, type) == kBlockCols * type_bytes(type);
+}
+
+// Division of 32-bit numbers by one that a launch does not change (Granlund and Montgomery, "Division by invariant
+// integers using multiplication", PLDI 1994).
+struct Divisor {
+  uint32_t by, magic, shift1, shift2;
+};
+static inline Divisor divisor(uint32_t d) {
+  int l = 0;
+  while (l < 32 && ((uint64_t)1 << l) < d) ++l;
+  const uint64_t m = ((((uint64_t)1 << l) - d) << 32) / d + 1;
+  return {d, (uint32_t)m, (uint32_t)(l < 1 ? l : 1), (uint32_t)(l > 1 ? l - 1 : 0)};
 }
 
 #ifdef __CUDACC__
+
+__device__ __forceinline__ uint32_t divide(uint32_t n, const Divisor& d) {
+  const uint32_t t = __umulhi(d.magic, n);
+  return (t + ((n - t) >> d.shift1)) >> d.shift2;
+}
 
 struct PhiloxKey { uint32_t k0, k1, offset_lo, offset_hi; };
 
@@ -87,10 +108,16 @@ __device__ __forceinline__ void drop_block(float (&x)[kBlockCols], const PhiloxK
                                            uint32_t block, uint32_t row) {
   const uint4 w = philox(make_uint4(block, row, k.offset_lo, k.offset_hi), k.k0, k.k1);
   const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+  if (drop_below > 0xffffu) {  // all of them
+#pragma unroll
+    for (int j = 0; j < kBlockCols; ++j) x[j] = 0.0f;
+    return;
+  }
+  const uint32_t top = drop_below << 16;  // halves are compared where they lie high in a word
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    x[2 * j] = (word[j] & 0xffffu) >= drop_below ? x[2 * j] * factor : 0.0f;
-    x[2 * j + 1] = (word[j] >> 16) >= drop_below ? x[2 * j + 1] * factor : 0.0f;
+    x[2 * j] = (word[j] << 16) >= top ? x[2 * j] * factor : 0.0f;
+    x[2 * j + 1] = word[j] >= top ? x[2 * j + 1] * factor : 0.0f;
   }
 }
 
@@ -98,6 +125,25 @@ __device__ __forceinline__ void drop_block(float (&x)[kBlockCols], const PhiloxK
 template <typename T> constexpr int block_words() { return kBlockCols * (int)sizeof(T) / 4; }
 
 template <int W> struct Words { uint32_t w[W]; };
+
+// Whole blocks that begin where a block can be moved at once.
+__device__ __forceinline__ void load_block(const void* p, Words<4>& v) {
+  asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]) : "l"(p));
+}
+__device__ __forceinline__ void load_block(const void* p, Words<8>& v) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void store_block(void* p, const Words<4>& v) {
+  *static_cast<uint4*>(p) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+}
+__device__ __forceinline__ void store_block(void* p, const Words<8>& v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v.w[0]), "r"(v.w[1]), "r"(v.w[2]),
+               "r"(v.w[3]), "r"(v.w[4]), "r"(v.w[5]), "r"(v.w[6]), "r"(v.w[7])
+               : "memory");
+}
 
 // Loads of what no other thread of the launch writes (an in-place call reads a value before it writes it, in one thread).
 // width: access_bytes of the matrix; cols: columns of the row from the block on, eight of a whole block.
@@ -116,7 +162,7 @@ __device__ __forceinline__ void load_words(const T* p, int width, int cols, Word
       for (int i = 0; i < kBlockCols; ++i)
         if (i < cols) v.w[i / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
     }
-  } else if (width == 16) {
+  } else if (width >= 16) {
 #pragma unroll
     for (int i = 0; i < W; i += 4) {
       const uint4 t = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i);
@@ -131,10 +177,19 @@ __device__ __forceinline__ void load_words(const T* p, int width, int cols, Word
   } else if (width == 4) {
 #pragma unroll
     for (int i = 0; i < W; ++i) v.w[i] = reinterpret_cast<const uint32_t*>(p)[i];
-  } else {
-    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+  } else if constexpr (sizeof(T) == 2) {
+    if ((uintptr_t)p & 2u) {  // the first value, three words, the last value
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+      const uint32_t* m = reinterpret_cast<const uint32_t*>(h + 1);
+      const uint32_t first = h[0], m0 = m[0], m1 = m[1], m2 = m[2], last = h[7];
+      v.w[0] = first | m0 << 16;
+      v.w[1] = __funnelshift_r(m0, m1, 16);
+      v.w[2] = __funnelshift_r(m1, m2, 16);
+      v.w[3] = m2 >> 16 | last << 16;
+    } else {
 #pragma unroll
-    for (int i = 0; i < W; ++i) v.w[i] = (uint32_t)h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
+      for (int i = 0; i < W; ++i) v.w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    }
   }
 }
 
@@ -151,7 +206,7 @@ __device__ __forceinline__ void store_words(T* p, int width, int cols, const Wor
       for (int i = 0; i < kBlockCols; ++i)
         if (i < cols) reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(v.w[i / 2] >> (16 * (i & 1)));
     }
-  } else if (width == 16) {
+  } else if (width >= 16) {
 #pragma unroll
     for (int i = 0; i < W; i += 4)
       *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(p) + i) = make_uint4(v.w[i], v.w[i + 1], v.w[i + 2], v.w[i + 3]);
@@ -162,7 +217,7 @@ __device__ __forceinline__ void store_words(T* p, int width, int cols, const Wor
   } else if (width == 4) {
 #pragma unroll
     for (int i = 0; i < W; ++i) reinterpret_cast<uint32_t*>(p)[i] = v.w[i];
-  } else {
+  } else if constexpr (sizeof(T) == 2) {
     uint16_t* h = reinterpret_cast<uint16_t*>(p);
 #pragma unroll
     for (int i = 0; i < W; ++i) {

@@ -1,8 +1,9 @@
 // Scaled embedding lookup with dropout, and dropout of rows: out[i, c] = keep(i, c) * factor * row_i[c].
 //
-// A flat list of blocks of eight columns, rows one after the other, U of them to a thread: reads and writes of a warp are
-// neighbours whatever the width, one row of one token is spread over the CTAs that it needs, and no lane idles but in the
-// last CTA.  Bound by memory; with dropout of 16-bit values the generator takes about as long as the values' way.
+// Rows whose blocks of eight columns can be moved at once (rows_kernel): a thread has one block of U rows that follow one
+// another, so that U rows are on their way, the column's part of the generator's first rounds is computed once, and a warp
+// moves 512 bytes or 1 KB of a row at a time.  Other rows (ragged_kernel): a flat list of blocks, 32 neighbours to a warp,
+// whose values go through shared memory where they cannot leave at once, so that a warp stores whole lines.
 #include "droprows.cuh"
 
 namespace hb {
@@ -11,22 +12,26 @@ int* device_error_word();  // runtime.cu
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kRows = 4;  // of a thread
 
 struct LookupArgs {
   const void* src;
   void* dst;
   const void* ids;      // null: row i of src for row i
-  int64_t n, rows, src_stride, dst_stride;
+  int64_t first;        // row of the launch's first row
+  int64_t rows, src_stride, dst_stride;
   int64_t padding;
-  uint32_t cols, blocks;  // of a row
-  uint32_t magic;       // ceil(2^32 / blocks), 0 where it does not divide exactly
+  uint32_t n, cols;     // rows of the launch
+  Divisor blocks;       // of a row
   int idx_bytes;
   int src_width, dst_width;
+  bool dst_linear;      // a row of dst begins where the one before ends
   Dropout drop;
   int* err;
 };
 
-__device__ __forceinline__ int64_t token_row(const LookupArgs& a, int64_t i) {
+// Row of the source for row i of the output, -1: zeros.
+__device__ __forceinline__ int64_t source_row(const LookupArgs& a, int64_t i) {
   if (!a.ids) return i;
   const int64_t id = a.idx_bytes == 8 ? static_cast<const int64_t*>(a.ids)[i] : static_cast<const int32_t*>(a.ids)[i];
   if (id == a.padding) return -1;
@@ -37,22 +42,72 @@ __device__ __forceinline__ int64_t token_row(const LookupArgs& a, int64_t i) {
   return id;
 }
 
+template <typename TI>
+__device__ __forceinline__ void scaled_values(const LookupArgs& a, const Words<block_words<TI>()>& in, const PhiloxKey& key,
+                                              uint32_t block, uint32_t row, float (&x)[kBlockCols]) {
+  values_of<TI>(in, x);
+  if (a.drop.drop_below) {
+    drop_block(x, key, a.drop.drop_below, a.drop.factor, block, row);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kBlockCols; ++i) x[i] *= a.drop.factor;
+  }
+}
+
 template <typename TI, typename TO, int U>
-__global__ void __launch_bounds__(kThreads) embedding_kernel(const LookupArgs a) {
-  const uint64_t first = (uint64_t)blockIdx.x * (kThreads * U);
-  const uint64_t row0 = first >> 32 ? first / a.blocks : (uint32_t)first / a.blocks;
-  const uint32_t rest = (uint32_t)(first - row0 * a.blocks);
-  int64_t row[U], from[U];
-  uint32_t block[U];
+__global__ void __launch_bounds__(kThreads) rows_kernel(const LookupArgs a) {
+  const uint32_t t = blockIdx.x * kThreads + threadIdx.x;
+  const uint32_t group = divide(t, a.blocks), block = t - group * a.blocks.by;
+  const uint32_t row0 = group * U;
+  if (row0 >= a.n) return;
+  int64_t from[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) from[u] = row0 + u < a.n ? source_row(a, a.first + row0 + u) : -1;
+  Words<block_words<TI>()> in[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const uint32_t at = rest + u * kThreads + threadIdx.x;
-    const uint32_t q = a.magic ? __umulhi(at, a.magic) : at / a.blocks;
-    block[u] = at - q * a.blocks;
-    row[u] = (int64_t)row0 + q;
-    from[u] = row[u] < a.n ? token_row(a, row[u]) : -1;
+    if (from[u] >= 0) {
+      load_block(static_cast<const TI*>(a.src) + from[u] * a.src_stride + block * kBlockCols, in[u]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < block_words<TI>(); ++i) in[u].w[i] = 0u;
+    }
   }
+  PhiloxKey key = {};
+  if (a.drop.drop_below) key = philox_key(a.drop);
+  TO* to = static_cast<TO*>(a.dst) + (a.first + row0) * a.dst_stride + block * kBlockCols;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (row0 + u >= a.n) break;
+    float x[kBlockCols];
+    scaled_values<TI>(a, in[u], key, block, (uint32_t)(a.first + row0 + u), x);
+    if (from[u] < 0) {
+#pragma unroll
+      for (int i = 0; i < kBlockCols; ++i) x[i] = 0.0f;  // (not -0 of a negative scale)
+    }
+    Words<block_words<TO>()> out;
+    words_of<TO>(x, out);
+    store_block(to + u * a.dst_stride, out);
+  }
+}
+
+__device__ __forceinline__ int staged_at(int e) { return e + (e >> 3); }
+
+template <typename TI, typename TO, int U>
+__global__ void __launch_bounds__(kThreads) ragged_kernel(const LookupArgs a) {
+  __shared__ float s_row[kThreads / 32][32 * (kBlockCols + 1)];
+  float* staged = s_row[threadIdx.x >> 5];
+  const int lane = threadIdx.x & 31;
+  uint32_t row[U], block[U];
+  int64_t from[U];
   Words<block_words<TI>()> in[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t t = (blockIdx.x * U + u) * kThreads + threadIdx.x;
+    row[u] = divide(t, a.blocks);
+    block[u] = t - row[u] * a.blocks.by;
+    from[u] = row[u] < a.n ? source_row(a, a.first + row[u]) : -1;
+  }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const uint32_t c = block[u] * kBlockCols;
@@ -61,52 +116,87 @@ __global__ void __launch_bounds__(kThreads) embedding_kernel(const LookupArgs a)
   }
   PhiloxKey key = {};
   if (a.drop.drop_below) key = philox_key(a.drop);
+  const bool direct = !a.dst_linear || a.dst_width == kBlockCols * (int)sizeof(TO);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    if (row[u] >= a.n) continue;
-    float x[kBlockCols];
-    if (from[u] >= 0) {
-      values_of<TI>(in[u], x);
-      if (a.drop.drop_below) {
-        drop_block(x, key, a.drop.drop_below, a.drop.factor, block[u], (uint32_t)row[u]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kBlockCols; ++i) x[i] *= a.drop.factor;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kBlockCols; ++i) x[i] = 0.0f;
-    }
-    Words<block_words<TO>()> out;
-    words_of<TO>(x, out);
+    const bool valid = row[u] < a.n;
     const uint32_t c = block[u] * kBlockCols;
-    store_words(static_cast<TO*>(a.dst) + row[u] * a.dst_stride + c, a.dst_width, a.cols - c, out);
+    const int64_t at = a.first + row[u];
+    float x[kBlockCols];
+#pragma unroll
+    for (int i = 0; i < kBlockCols; ++i) x[i] = 0.0f;
+    if (from[u] >= 0) scaled_values<TI>(a, in[u], key, block[u], (uint32_t)at, x);
+    if (direct) {
+      if (valid) {
+        Words<block_words<TO>()> out;
+        words_of<TO>(x, out);
+        store_words(static_cast<TO*>(a.dst) + at * a.dst_stride + c, a.dst_width, a.cols - c, out);
+      }
+      continue;
+    }
+    // the warp's blocks are one stretch of memory: values [0, length) from `begin` on
+    const int mine = !valid ? 0 : a.cols - c < kBlockCols ? (int)(a.cols - c) : kBlockCols;
+    const int64_t place = at * a.cols + c;
+    const int64_t begin = __shfl_sync(0xffffffffu, place, 0);
+    const int length = __reduce_max_sync(0xffffffffu, valid ? (int)(place - begin) + mine : 0);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kBlockCols; ++i)
+      if (i < mine) staged[staged_at((int)(place - begin) + i)] = x[i];
+    __syncwarp();
+    TO* to = static_cast<TO*>(a.dst) + begin;
+    if constexpr (sizeof(TO) == 4) {
+      for (int e = lane; e < length; e += 32) to[e] = staged[staged_at(e)];
+    } else {
+      const int odd = (int)(((uintptr_t)to >> 1) & 1u);  // words of memory begin one value earlier
+      for (int e = 2 * lane - odd; e < length; e += 64) {
+        const float lo = e >= 0 ? staged[staged_at(e)] : 0.0f, hi = e + 1 < length ? staged[staged_at(e + 1)] : 0.0f;
+        uint32_t w;
+        if constexpr (std::is_same_v<TO, __half>) {
+          const __half2 h = __floats2half2_rn(lo, hi);
+          w = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+          w = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        if (e >= 0 && e + 1 < length) *reinterpret_cast<uint32_t*>(to + e) = w;
+        else if (e >= 0) *reinterpret_cast<uint16_t*>(to + e) = (uint16_t)w;
+        else *reinterpret_cast<uint16_t*>(to + e + 1) = (uint16_t)(w >> 16);
+      }
+    }
   }
 }
 
-int lookup(const char* who, LookupArgs a, int src_type, int dst_type, cudaStream_t st) {
-  if (a.n == 0) return HB_OK;
+int lookup(const char* who, LookupArgs a, int64_t n, int src_type, int dst_type, cudaStream_t st) {
+  if (n == 0) return HB_OK;
   a.err = device_error_word();
   HB_CHECK_ARG(a.err != nullptr, "%s: no error word on this device", who);
-  a.blocks = (a.cols + kBlockCols - 1) / kBlockCols;
-  // at * (magic * blocks - 2^32) < 2^32 for every local index: exact
-  const uint64_t top = (uint64_t)a.blocks + 4 * kThreads;
-  a.magic = a.blocks > 1 && top * a.blocks < ((uint64_t)1 << 32) ? (uint32_t)((((uint64_t)1 << 32) + a.blocks - 1) / a.blocks) : 0;
+  const uint32_t blocks = (a.cols + kBlockCols - 1) / kBlockCols;
+  a.blocks = divisor(blocks);
   a.src_width = access_bytes(a.src, a.src_stride, src_type);
   a.dst_width = access_bytes(a.dst, a.dst_stride, dst_type);
-  const int64_t items = a.n * a.blocks;
-  const bool few = items <= (int64_t)sm_count() * kThreads * 8;
-  const int64_t grid = ceil_div(items, (int64_t)kThreads * (few ? 1 : 4));
-  HB_CHECK_ARG(grid < ((int64_t)1 << 31), "%s: more blocks than a launch holds", who);
-  return with_type(src_type, [&](auto ti) {
-    return with_type(dst_type, [&](auto to) -> int {
-      using TI = decltype(ti);
-      using TO = decltype(to);
-      if (few) HB_LAUNCH((embedding_kernel<TI, TO, 1>), (int)grid, kThreads, 0, st, a);
-      else HB_LAUNCH((embedding_kernel<TI, TO, 4>), (int)grid, kThreads, 0, st, a);
-      return HB_OK;
+  a.dst_linear = a.dst_stride == a.cols || n == 1;
+  const bool whole = whole_blocks(a.src, a.src_stride, src_type, a.cols) && whole_blocks(a.dst, a.dst_stride, dst_type, a.cols);
+  const bool few = n * blocks <= (int64_t)sm_count() * kThreads * 8;
+  const int64_t most = (((int64_t)1 << 31) / blocks) & ~(int64_t)(kRows - 1);  // rows whose blocks count in 32 bits
+  for (int64_t first = 0; first < n; first += most) {
+    a.first = first;
+    a.n = (uint32_t)(n - first < most ? n - first : most);
+    const int rc = with_type(src_type, [&](auto ti) {
+      return with_type(dst_type, [&](auto to) -> int {
+        using TI = decltype(ti);
+        using TO = decltype(to);
+        auto grid = [&](int64_t items, int each) { return (int)ceil_div(items, (int64_t)kThreads * each); };
+        if (whole && few) HB_LAUNCH((rows_kernel<TI, TO, 1>), grid((int64_t)a.n * blocks, 1), kThreads, 0, st, a);
+        else if (whole) HB_LAUNCH((rows_kernel<TI, TO, kRows>), grid(ceil_div(a.n, kRows) * blocks, 1), kThreads, 0, st, a);
+        else if (few) HB_LAUNCH((ragged_kernel<TI, TO, 1>), grid((int64_t)a.n * blocks, 1), kThreads, 0, st, a);
+        else HB_LAUNCH((ragged_kernel<TI, TO, 2>), grid((int64_t)a.n * blocks, 2), kThreads, 0, st, a);
+        return HB_OK;
+      });
     });
-  });
+    if (rc != HB_OK) return rc;
+  }
+  return HB_OK;
 }
 
 }  // namespace
@@ -134,14 +224,13 @@ int hb_embedding(const void* weight, int weight_type, int64_t weight_stride, int
   a.src = weight;
   a.dst = out;
   a.ids = ids;
-  a.n = n;
   a.rows = num_rows;
   a.src_stride = weight_stride;
   a.dst_stride = out_stride;
   a.padding = padding_idx;
   a.cols = (uint32_t)dim;
   a.idx_bytes = idx_bytes;
-  return lookup("hb_embedding", a, weight_type, out_type, (cudaStream_t)stream);
+  return lookup("hb_embedding", a, n, weight_type, out_type, (cudaStream_t)stream);
 }
 
 int hb_dropout(const void* x, int x_type, int64_t x_stride, int64_t n, int64_t dim, double scale, const hb_drop_t* drop,
@@ -158,11 +247,11 @@ int hb_dropout(const void* x, int x_type, int64_t x_stride, int64_t n, int64_t d
                "hb_dropout: the output is neither apart from the input nor the input itself");
   a.src = x;
   a.dst = y;
-  a.n = a.rows = n;
+  a.rows = n;
   a.src_stride = x_stride;
   a.dst_stride = y_stride;
   a.cols = (uint32_t)dim;
-  return lookup("hb_dropout", a, x_type, y_type, (cudaStream_t)stream);
+  return lookup("hb_dropout", a, n, x_type, y_type, (cudaStream_t)stream);
 }
 
 }  // extern "C"
