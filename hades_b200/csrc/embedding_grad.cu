@@ -3,9 +3,10 @@
 //
 // The tokens are sorted with their positions (runs.cu), and the sorted entries are cut into pieces of equal length, whatever
 // token they hold: a token that is a tenth of all positions costs no warp more than another.  32 lanes take 256 columns of a
-// piece, sums stay in registers, and a row leaves as soon as its token ends.  What of a token lies in two pieces or more is
-// left as fp32 partial rows and added up by a second launch, in the order of the pieces, so that the result depends on
-// the sizes of the call alone.
+// piece; rows come through a ring of asynchronous copies in shared memory (a lane copies and reads its own eight columns, so
+// that nothing is waited for but the copy), sums stay in registers, and a row leaves as soon as its token ends.  What of a
+// token lies in two pieces or more is left as fp32 partial rows and added up by a second launch, in the order of the pieces,
+// so that the result depends on the sizes of the call alone.
 #include "droprows.cuh"
 #include "runs.cuh"
 
@@ -15,32 +16,67 @@ int* device_error_word();  // runtime.cu
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
-constexpr int64_t kNoRow = -1;
+constexpr int kWindow = 256;   // sorted entries of a warp
+constexpr int kStages = 8;     // rows of a warp's ring
+constexpr int kSumWarps = 4;   // of a CTA
+constexpr uint32_t kHead = 0x80000000u;
 
 // ---- tokens as sort keys: what takes no part (padding, ids outside of the table) sorts last, as num_rows --------------
+struct Zeros {
+  char* p;          // rows to zero in the same launch, null: none
+  int64_t rows, row_bytes, stride_bytes;
+  int width;        // bytes at a time: as all rows allow; of a single one 16, but for its ends
+};
+
 template <typename Id>
 __global__ void __launch_bounds__(kThreads) token_keys_kernel(const Id* ids, int64_t n, int64_t padding, int64_t num_rows,
-                                                              int64_t* keys, int* err) {
-  for (int64_t i = blockIdx.x * (int64_t)kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
+                                                              int64_t* keys, int* err, Zeros z) {
+  const int64_t at = blockIdx.x * (int64_t)kThreads + threadIdx.x, threads = (int64_t)gridDim.x * kThreads;
+  for (int64_t i = at; i < n; i += threads) {
     const int64_t id = ids[i];
     const bool inside = id >= 0 && id < num_rows;
     if (!inside && id != padding) atomicExch(err, HB_ERR_INVALID);
     keys[i] = inside && id != padding ? id : num_rows;
   }
+  if (!z.p) return;
+  if (z.rows == 1) {
+    char *const end = z.p + z.row_bytes, *from = reinterpret_cast<char*>(((uintptr_t)z.p + 15) & ~(uintptr_t)15);
+    if (from > end) from = end;
+    char* to = from + ((end - from) & ~(int64_t)15);
+    for (char* p = from + at * 16; p < to; p += threads * 16) *reinterpret_cast<uint4*>(p) = make_uint4(0u, 0u, 0u, 0u);
+    if (at < 8) {
+      if (z.p + 2 * at < from) reinterpret_cast<uint16_t*>(z.p)[at] = 0;
+      if (to + 2 * at < end) reinterpret_cast<uint16_t*>(to)[at] = 0;
+    }
+    return;
+  }
+  const int64_t per_row = z.row_bytes / z.width, items = z.rows * per_row;
+  for (int64_t i = at; i < items; i += threads) {
+    char* p = z.p + i / per_row * z.stride_bytes + i % per_row * z.width;
+    if (z.width == 16) *reinterpret_cast<uint4*>(p) = make_uint4(0u, 0u, 0u, 0u);
+    else if (z.width == 8) *reinterpret_cast<uint2*>(p) = make_uint2(0u, 0u);
+    else if (z.width == 4) *reinterpret_cast<uint32_t*>(p) = 0u;
+    else *reinterpret_cast<uint16_t*>(p) = 0;
+  }
 }
 
 // ---- sums ---------------------------------------------------------------------------------------------------------------
+struct Link {        // of a piece whose last token goes on behind it and does not come from before it
+  int64_t row;       // of the output
+  int64_t pieces;    // behind this one that the token lies in; 0: no such token
+};
+
 struct GradArgs {
   hb_runs_t runs;
   const void* grads;
   int64_t grad_stride;
-  int grad_width;
+  int chunk;                     // bytes of a copy: 16, 8, 4; 2: copies of 4 that may begin 2 bytes early
   uint32_t cols, blocks, tiles;  // columns, blocks of eight, tiles of `lanes` blocks
-  int lanes;                     // of a unit, a power of two
-  int64_t per;                   // sorted entries of a piece, a multiple of 8
+  int lanes;                     // of a unit, a power of two; a warp holds 32 / lanes units, pieces that follow one another
+  int per;                       // sorted entries of a piece, a multiple of 8
   int64_t pieces;
-  float* parts;                  // [pieces][2][tiles * lanes * 8]: what the piece has of the token before, of the token behind
+  float* parts;                  // [pieces][2][tiles * lanes * 8]: what a piece has of the token before, of the token behind
+  Link* links;                   // [pieces]
   Dropout drop;
   void* out;
   int64_t out_stride;
@@ -51,21 +87,16 @@ struct GradArgs {
   int64_t* num_unique;           // nullable
 };
 
-// Entries and runs that take part: the run of what does not is the last one.
-__device__ __forceinline__ void taking_part(const GradArgs& a, int64_t& entries, int64_t& runs) {
-  runs = *a.runs.num_runs;
-  entries = runs_valid_entries(a.runs);
-  if (runs > 0 && a.runs.uniq_ids[runs - 1] >= a.num_rows) entries = a.runs.run_start[--runs];
-  if (runs <= 0) entries = 0;
+__device__ __forceinline__ float* part_at(const GradArgs& a, int64_t piece, int behind, uint32_t block) {
+  return a.parts + ((piece * 2 + behind) * (int64_t)(a.tiles * a.lanes) + block) * kBlockCols;
 }
-
-__device__ __forceinline__ int64_t part_at(const GradArgs& a, int64_t piece, int behind, uint32_t block) {
-  return ((piece * 2 + behind) * (int64_t)(a.tiles * a.lanes) + block) * kBlockCols;
+__device__ __forceinline__ void put_part(float* p, const float (&x)[kBlockCols]) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
 }
 
 template <typename TO>
-__device__ __forceinline__ void put_row(const GradArgs& a, int64_t run, uint32_t block, float (&x)[kBlockCols]) {
-  const int64_t row = a.by_run ? run : a.runs.uniq_ids[run];
+__device__ __forceinline__ void put_row(const GradArgs& a, int64_t row, uint32_t block, float (&x)[kBlockCols]) {
   const uint32_t c = block * kBlockCols;
   TO* p = static_cast<TO*>(a.out) + row * a.out_stride + c;
   Words<block_words<TO>()> w;
@@ -83,126 +114,227 @@ __device__ __forceinline__ void put_row(const GradArgs& a, int64_t run, uint32_t
   store_words(p, a.out_width, a.cols - c, w);
 }
 
-template <typename TG, typename TO>
-__global__ void __launch_bounds__(kThreads) grad_sum_kernel(const GradArgs a) {
-  constexpr int kFly = sizeof(TG) == 4 ? 4 : 8;  // rows on their way at once
-  const int64_t unit = (blockIdx.x * (int64_t)kThreads + threadIdx.x) / a.lanes;
-  const int64_t piece = unit / a.tiles;
-  const uint32_t block = (uint32_t)(unit - piece * a.tiles) * a.lanes + (threadIdx.x & (a.lanes - 1));
-  int64_t entries, runs;
-  taking_part(a, entries, runs);
-  if (a.num_unique && blockIdx.x == 0 && threadIdx.x == 0) *a.num_unique = runs;
-  const int64_t begin = piece * a.per, end = begin + a.per < entries ? begin + a.per : entries;
-  if (begin >= end || block >= a.blocks) return;
+// ---- a lane's block of a row through shared memory: copy i of a stage at (i * 32 + lane) * bytes ------------------------
+template <typename T> constexpr int stage_bytes() { return 32 * (sizeof(T) == 4 ? 32 : 20); }
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copy_async_part(uint32_t to, const void* from, int bytes) {  // the rest of 4: zeros
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+
+// bytes: of the row from p on (a multiple of the chunk, whatever it is)
+template <typename T, bool WIDE>
+__device__ __forceinline__ void copy_block(uint32_t stage, const T* p, int chunk, int bytes, int lane) {
+  constexpr int B = kBlockCols * (int)sizeof(T);
+  const char* from = reinterpret_cast<const char*>(p);
+  if (WIDE) {
+#pragma unroll
+    for (int i = 0; i < B / 16; ++i)
+      if (i == 0 || i * 16 < bytes) copy_async<16>(stage + (i * 32 + lane) * 16, from + i * 16);
+  } else if (chunk == 8) {
+#pragma unroll
+    for (int i = 0; i < B / 8; ++i)
+      if (i * 8 < bytes) copy_async<8>(stage + (i * 32 + lane) * 8, from + i * 8);
+  } else if (chunk == 4) {
+#pragma unroll
+    for (int i = 0; i < B / 4; ++i)
+      if (i * 4 < bytes) copy_async<4>(stage + (i * 32 + lane) * 4, from + i * 4);
+  } else if constexpr (sizeof(T) == 2) {
+    // words of memory, the first of which may begin with the value before (of the row before, or, as an allocation
+    // begins at a word, at least of the same allocation); the last is cut where the row ends
+    const int early = (int)((uintptr_t)p & 2u);
+    const int all = early + (bytes < B ? bytes : B);
+#pragma unroll
+    for (int i = 0; i < 5; ++i)
+      if (i * 4 < all) copy_async_part(stage + (i * 32 + lane) * 4, from - early + i * 4, all - i * 4 < 4 ? all - i * 4 : 4);
+  }
+}
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ void copied_block(const char* stage, const T* p, int chunk, int lane, Words<block_words<T>()>& v) {
+  constexpr int W = block_words<T>();
+  if (WIDE) {
+#pragma unroll
+    for (int i = 0; i < W / 4; ++i) {
+      const uint4 t = reinterpret_cast<const uint4*>(stage)[i * 32 + lane];
+      v.w[4 * i] = t.x; v.w[4 * i + 1] = t.y; v.w[4 * i + 2] = t.z; v.w[4 * i + 3] = t.w;
+    }
+  } else if (chunk == 8) {
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) {
+      const uint2 t = reinterpret_cast<const uint2*>(stage)[i * 32 + lane];
+      v.w[2 * i] = t.x; v.w[2 * i + 1] = t.y;
+    }
+  } else {
+    const uint32_t* s = reinterpret_cast<const uint32_t*>(stage);
+#pragma unroll
+    for (int i = 0; i < W; ++i) v.w[i] = s[i * 32 + lane];
+    if constexpr (sizeof(T) == 2) {
+      if (chunk == 2 && ((uintptr_t)p & 2u)) {
+        const uint32_t last = s[4 * 32 + lane];
+#pragma unroll
+        for (int i = 0; i < W; ++i) v.w[i] = __funnelshift_r(v.w[i], i + 1 < W ? v.w[i + 1] : last, 16);
+      }
+    }
+  }
+}
+
+// WIDE: copies of 16 bytes.
+template <typename TG, typename TO, bool WIDE>
+__global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs a) {
+  begin_after_previous();
+  __shared__ alignas(16) char s_ring[kSumWarps][kStages][stage_bytes<TG>()];
+  __shared__ int64_t s_row[kSumWarps][kWindow];          // of the output, for every entry
+  __shared__ uint32_t s_entry[kSumWarps][kWindow + 1];   // its position; kHead: a token begins
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t index = blockIdx.x * (int64_t)kSumWarps + warp;
+  if (a.num_unique && blockIdx.x == 0 && threadIdx.x == 0) {  // (the run of what takes no part is the last one)
+    const int64_t runs = *a.runs.num_runs;
+    *a.num_unique = runs > 0 && a.runs.uniq_ids[runs - 1] >= a.num_rows ? runs - 1 : runs;
+  }
+  const int units = 32 / a.lanes, length = units * a.per;
+  const int64_t first = index / a.tiles, begin = first * length;  // (one tile where a warp holds several units)
+  if (begin >= a.runs.n) return;
+
+  // the warp's entries, and the one behind them; entries that take no part count as heads, and lie behind all others
+  const int64_t valid_entries = runs_valid_entries(a.runs);
+  int valid = 0;
+  for (int i0 = 0; i0 <= length; i0 += 32) {
+    const int i = i0 + lane;
+    const int64_t j = begin + i;
+    const bool in = i <= length && j < valid_entries;
+    const bool head = in && a.runs.head[j] != 0;
+    const uint32_t octet = (__ballot_sync(0xffffffffu, head) >> (lane & ~7)) & 0xffu;
+    bool part = false;
+    if (in) {
+      const int64_t run = a.runs.base8[j >> 3] + __popc(octet & ((2u << (lane & 7)) - 1u)) - 1;
+      const int64_t token = a.runs.uniq_ids[run];
+      part = token < a.num_rows;
+      if (i < length) s_row[warp][i] = a.by_run ? run : token;
+      s_entry[warp][i] = part ? a.runs.perm[j] | (head ? kHead : 0u) : kHead;
+    } else if (i <= length) {
+      s_entry[warp][i] = kHead;
+    }
+    valid += __popc(__ballot_sync(0xffffffffu, part && i < length));
+  }
+  __syncwarp();
+
+  const int unit = lane / a.lanes;
+  const int64_t piece = first * units + unit;
+  const uint32_t block = (uint32_t)(index - first * a.tiles) * a.lanes + (lane & (a.lanes - 1));
   const uint32_t c = block * kBlockCols;
+  const bool leads = block == 0;  // writes the piece's link
+  const int from = unit * a.per, to = from + a.per < valid ? from + a.per : valid;
+  if (from >= to || block >= a.blocks) {
+    if (leads && piece < a.pieces) a.links[piece] = Link{0, 0};
+    return;
+  }
+  const uint32_t* entry = s_entry[warp];
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_ring[warp][0]);
+  const TG* grads = static_cast<const TG*>(a.grads) + c;
+  const int bytes = (int)(a.cols - c) * (int)sizeof(TG);
+  auto row_of = [&](int e) { return grads + (int64_t)(entry[e] & ~kHead) * a.grad_stride; };
+  auto issue = [&](int e, int stage) {
+    if (e < to) {
+      copy_block<TG, WIDE>(ring + stage * stage_bytes<TG>(), row_of(e), a.chunk, bytes, lane);
+      if (a.accumulate && (entry[e] & kHead))
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<TO*>(a.out) + s_row[warp][e] * a.out_stride + c));
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int s = 0; s < kStages; ++s) issue(from + s, s);
   PhiloxKey key = {};
   if (a.drop.drop_below) key = philox_key(a.drop);
   float sum[kBlockCols];
 #pragma unroll
   for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
-  int64_t run = a.runs.base8[begin >> 3] - 1;  // (of the entry before, which a head at `begin` ends)
-  bool before = a.runs.head[begin] == 0;       // the sum belongs to a token that began before the piece
-  bool any = before;
-  for (int64_t j0 = begin; j0 < end; j0 += kFly) {
-    uint32_t pos[kFly];
-    uint8_t head[kFly];
-    Words<block_words<TG>()> in[kFly];
+  bool before = !(entry[from] & kHead);  // the sum belongs to a token that began before the piece
+  int stage = 0;
+  for (int e = from; e < to; ++e) {
+    if (e > from && (entry[e] & kHead)) {  // the token before ends
+      if (before) put_part(part_at(a, piece, 0, block), sum);
+      else put_row<TO>(a, s_row[warp][e - 1], block, sum);
 #pragma unroll
-    for (int k = 0; k < kFly; ++k) {
-      const int64_t j = j0 + k < end ? j0 + k : end - 1;
-      pos[k] = a.runs.perm[j];
-      head[k] = a.runs.head[j];
+      for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
+      before = false;
     }
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    Words<block_words<TG>()> in;
+    copied_block<TG, WIDE>(s_ring[warp][stage], row_of(e), a.chunk, lane, in);
+    float x[kBlockCols];
+    values_of<TG>(in, x);
+    if (a.drop.drop_below) drop_block(x, key, a.drop.drop_below, 1.0f, block, entry[e] & ~kHead);
 #pragma unroll
-    for (int k = 0; k < kFly; ++k)
-      load_words(static_cast<const TG*>(a.grads) + (int64_t)pos[k] * a.grad_stride + c, a.grad_width, a.cols - c, in[k]);
-#pragma unroll
-    for (int k = 0; k < kFly; ++k) {
-      if (j0 + k >= end) break;
-      if (head[k]) {
-        if (any) {
-          if (before) {
-            float* p = a.parts + part_at(a, piece, 0, block);
-            *reinterpret_cast<float4*>(p) = make_float4(sum[0], sum[1], sum[2], sum[3]);
-            *reinterpret_cast<float4*>(p + 4) = make_float4(sum[4], sum[5], sum[6], sum[7]);
-          } else {
-            put_row<TO>(a, run, block, sum);
-          }
-#pragma unroll
-          for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
-        }
-        ++run;
-        before = false;
-        any = true;
-      }
-      float x[kBlockCols];
-      values_of<TG>(in[k], x);
-      if (a.drop.drop_below) drop_block(x, key, a.drop.drop_below, 1.0f, block, pos[k]);
-#pragma unroll
-      for (int i = 0; i < kBlockCols; ++i) sum[i] += x[i];
-    }
+    for (int i = 0; i < kBlockCols; ++i) sum[i] += x[i];
+    issue(e + kStages, stage);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
   }
-  const bool ends = end == entries || a.runs.head[end] != 0;  // its last token goes no further
-  if (ends && !before) {
-    put_row<TO>(a, run, block, sum);
+  const bool ends = (entry[to] & kHead) != 0;  // the last token goes no further
+  Link link{0, 0};
+  if (before) {
+    put_part(part_at(a, piece, 0, block), sum);
+  } else if (ends) {
+    put_row<TO>(a, s_row[warp][to - 1], block, sum);
   } else {
-    float* p = a.parts + part_at(a, piece, before ? 0 : 1, block);
-    *reinterpret_cast<float4*>(p) = make_float4(sum[0], sum[1], sum[2], sum[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(sum[4], sum[5], sum[6], sum[7]);
+    put_part(part_at(a, piece, 1, block), sum);
+    if (leads) {
+      const int64_t behind = begin + to;  // (a multiple of 8, as the piece is full)
+      const int64_t run = a.runs.base8[behind >> 3] - 1;
+      link = Link{s_row[warp][to - 1], (a.runs.run_start[run + 1] - 1) / a.per - piece};
+    }
   }
+  if (leads) a.links[piece] = link;
 }
 
-// Tokens that begin in one piece and end in another: the piece that they begin in adds up what the pieces have.  The warps
-// of a CTA take a stretch of the pieces each.
+// Tokens that begin in one piece and end in another: the parts of the pieces in order, a share of them for each of the
+// `shares` rows of threads of a CTA.
 template <typename TO>
-__global__ void __launch_bounds__(kThreads) grad_join_kernel(const GradArgs a) {
-  __shared__ float s_sum[kWarps][32][kBlockCols];
-  const int64_t piece = blockIdx.x / a.tiles;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t block = (uint32_t)(blockIdx.x - piece * a.tiles) * a.lanes + lane;
-  int64_t entries, runs;
-  taking_part(a, entries, runs);
-  const int64_t end = (piece + 1) * a.per;
-  if (end >= entries || a.runs.head[end]) return;
-  const int64_t run = a.runs.base8[end >> 3] - 1;
-  if (a.runs.run_start[run] < piece * a.per) return;
-  const int64_t stop = run + 1 < runs ? a.runs.run_start[run + 1] : entries;
-  const int64_t last = (stop - 1) / a.per, count = last - piece;  // and so many pieces behind this one
-  const int64_t share = (count + kWarps - 1) / kWarps;
+__global__ void __launch_bounds__(kThreads) grad_join_kernel(const GradArgs a, int width, int spans) {
+  begin_after_previous();
+  __shared__ float s_sum[kThreads][kBlockCols + 1];
+  const int64_t piece = blockIdx.x / spans;
+  const Link link = a.links[piece];
+  if (link.pieces == 0) return;
+  const uint32_t block = (uint32_t)(blockIdx.x - piece * spans) * width + threadIdx.x % width;
+  const int shares = kThreads / width, mine = threadIdx.x / width;
+  const int64_t count = link.pieces + 1, share = (count + shares - 1) / shares;
+  const int64_t from = mine * share, to = from + share < count ? from + share : count;
   float sum[kBlockCols];
 #pragma unroll
   for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
-  const bool mine = lane < a.lanes && block < a.blocks;
-  if (mine) {
-    auto add = [&](const float* p) {
+  if (block < a.blocks) {
+#pragma unroll 4
+    for (int64_t k = from; k < to; ++k) {
+      const float* p = part_at(a, piece + k, k == 0, block);
       const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 4);
       sum[0] += x.x; sum[1] += x.y; sum[2] += x.z; sum[3] += x.w;
       sum[4] += y.x; sum[5] += y.y; sum[6] += y.z; sum[7] += y.w;
-    };
-    if (warp == 0) add(a.parts + part_at(a, piece, 1, block));
-    int64_t from = piece + 1 + warp * share, to = from + share;
-    if (to > last + 1) to = last + 1;
-#pragma unroll 4
-    for (int64_t q = from; q < to; ++q) add(a.parts + part_at(a, q, 0, block));
+    }
   }
-  if (share * 1 < count) {  // (more than one warp had a part)
+  if (share < count) {
 #pragma unroll
-    for (int i = 0; i < kBlockCols; ++i) s_sum[warp][lane][i] = sum[i];
+    for (int i = 0; i < kBlockCols; ++i) s_sum[threadIdx.x][i] = sum[i];
     __syncthreads();
-    if (warp == 0)
-      for (int w = 1; w < kWarps; ++w)
+    if (mine == 0)
+      for (int w = 1; w < shares && w * share < count; ++w)
 #pragma unroll
-        for (int i = 0; i < kBlockCols; ++i) sum[i] += s_sum[w][lane][i];
+        for (int i = 0; i < kBlockCols; ++i) sum[i] += s_sum[w * width + threadIdx.x][i];
   }
-  if (warp == 0 && mine) put_row<TO>(a, run, block, sum);
+  if (mine == 0 && block < a.blocks) put_row<TO>(a, link.row, block, sum);
 }
 
 struct GradPlan {
-  int lanes;
+  int lanes, per;
   uint32_t blocks, tiles;
-  int64_t per, pieces;
+  int64_t pieces;
   int64_t* keys;
   float* parts;
+  Link* links;
   void* runs_ws;
   size_t runs_bytes, total;
 };
@@ -214,14 +346,15 @@ GradPlan make_plan(void* ws, int64_t n, int64_t dim) {
   p.lanes = 1;
   while (p.lanes < 32 && p.lanes < (int)p.blocks) p.lanes *= 2;
   p.tiles = (uint32_t)ceil_div(p.blocks, p.lanes);
-  const int64_t warps = (int64_t)sm_count() * 24;
-  const int64_t units = warps * (32 / p.lanes);
-  p.per = align_up((size_t)ceil_div(m * p.tiles, units), 8);
-  if (p.per > 256) p.per = 256;
+  const int units = 32 / p.lanes;
+  const int64_t warps = (int64_t)sm_count() * 16;
+  const int64_t per = (int64_t)align_up((size_t)ceil_div(m * p.tiles, warps * units), 8);
+  p.per = (int)(per > kWindow / units ? kWindow / units : per);
   p.pieces = ceil_div(m, p.per);
   Carver cv(ws ? ws : (void*)256);
   p.keys = cv.take<int64_t>(m);
   p.parts = cv.take<float>((size_t)p.pieces * 2 * p.tiles * p.lanes * kBlockCols);
+  p.links = cv.take<Link>(p.pieces);
   p.runs_bytes = align_up(hb_runs_workspace_bytes(m), 256);
   p.runs_ws = cv.take<char>(p.runs_bytes);
   p.total = cv.used() + 256;
@@ -274,25 +407,26 @@ int grad(const Call& k) {
   }
   int* err = device_error_word();
   HB_CHECK_ARG(err != nullptr, "%s: no error word on this device", k.who);
+  Zeros z = {};
   if (!k.by_run && !k.accumulate && k.num_rows > 0) {
-    const size_t e = (size_t)type_bytes(k.out_type);
-    if (k.out_stride == k.dim || k.num_rows == 1)
-      HB_CUDA(cudaMemsetAsync(k.out, 0, (size_t)k.num_rows * k.dim * e, k.st));
-    else
-      HB_CUDA(cudaMemset2DAsync(k.out, k.out_stride * e, 0, k.dim * e, k.num_rows, k.st));
+    const int64_t e = type_bytes(k.out_type);
+    z = Zeros{static_cast<char*>(k.out), k.num_rows, k.dim * e, k.out_stride * e, 0};
+    if (k.num_rows == 1 || k.out_stride == k.dim) z = Zeros{z.p, 1, k.num_rows * k.dim * e, k.num_rows * k.dim * e, 0};
+    const uint64_t bits = (uint64_t)(uintptr_t)z.p | (uint64_t)z.row_bytes | (uint64_t)z.stride_bytes | 16u;
+    z.width = z.rows == 1 ? 16 : (int)(bits & (~bits + 1));
   }
-  if (k.n == 0) {
-    if (k.num_unique) HB_CUDA(cudaMemsetAsync(k.num_unique, 0, sizeof(int64_t), k.st));
-    return HB_OK;
-  }
-  const int64_t key_blocks = ceil_div(k.n, kThreads), cap = (int64_t)sm_count() * 8;
+  if (k.n == 0 && k.num_unique) HB_CUDA(cudaMemsetAsync(k.num_unique, 0, sizeof(int64_t), k.st));
+  if (k.n == 0 && !z.p) return HB_OK;
+  const int64_t items = z.p ? z.rows * ceil_div(z.row_bytes, z.width) : 0;
+  const int64_t key_blocks = ceil_div(k.n > items ? k.n : items, kThreads), cap = (int64_t)sm_count() * 8;
   const int key_grid = (int)(key_blocks < cap ? key_blocks : cap);
   if (k.idx_bytes == 8)
     HB_LAUNCH(token_keys_kernel<int64_t>, key_grid, kThreads, 0, k.st, static_cast<const int64_t*>(k.ids), k.n, k.padding,
-              k.num_rows, p.keys, err);
+              k.num_rows, p.keys, err, z);
   else
     HB_LAUNCH(token_keys_kernel<int32_t>, key_grid, kThreads, 0, k.st, static_cast<const int32_t*>(k.ids), k.n, k.padding,
-              k.num_rows, p.keys, err);
+              k.num_rows, p.keys, err, z);
+  if (k.n == 0) return HB_OK;
   int bits = 1;
   while ((((int64_t)1 << bits) - 1) <= k.num_rows) ++bits;  // keys up to num_rows lie below the sort's sentinel
   rc = runs_build(p.keys, k.n, nullptr, nullptr, 0, bits, nullptr, 0, nullptr, nullptr, k.uniq_ids, nullptr, nullptr, 0,
@@ -300,7 +434,9 @@ int grad(const Call& k) {
   if (rc != HB_OK) return rc;
   a.grads = k.grads;
   a.grad_stride = k.grad_stride;
-  a.grad_width = access_bytes(k.grads, k.grad_stride, k.grad_type);
+  const uint64_t ends = (uint64_t)(uintptr_t)k.grads | (uint64_t)(k.grad_stride * type_bytes(k.grad_type)) |
+                        (uint64_t)(k.dim * type_bytes(k.grad_type)) | 16u;
+  a.chunk = (int)(ends & (~ends + 1));
   a.cols = (uint32_t)k.dim;
   a.blocks = p.blocks;
   a.tiles = p.tiles;
@@ -308,6 +444,7 @@ int grad(const Call& k) {
   a.per = p.per;
   a.pieces = p.pieces;
   a.parts = p.parts;
+  a.links = p.links;
   a.out = k.out;
   a.out_stride = k.out_stride;
   a.out_width = access_bytes(k.out, k.out_stride, k.out_type);
@@ -315,17 +452,24 @@ int grad(const Call& k) {
   a.by_run = k.by_run;
   a.accumulate = k.accumulate;
   a.num_unique = k.num_unique;
-  const int64_t sum_grid = ceil_div(p.pieces * p.tiles * p.lanes, kThreads), join_grid = (p.pieces - 1) * p.tiles;
+  const int64_t warps = ceil_div(p.pieces, 32 / p.lanes) * p.tiles, sum_grid = ceil_div(warps, kSumWarps);
+  int width = 1;
+  while (width < kThreads && width < (int)p.blocks) width *= 2;
+  const int spans = (int)ceil_div(p.blocks, width);
+  const int64_t join_grid = (p.pieces - 1) * spans;
   HB_CHECK_ARG(sum_grid < ((int64_t)1 << 31) && join_grid < ((int64_t)1 << 31), "%s: more blocks than a launch holds", k.who);
   rc = with_type(k.grad_type, [&](auto tg) {
     return with_type(k.out_type, [&](auto to) -> int {
-      HB_LAUNCH((grad_sum_kernel<decltype(tg), decltype(to)>), (int)sum_grid, kThreads, 0, k.st, a);
+      using TG = decltype(tg);
+      using TO = decltype(to);
+      if (a.chunk == 16) HB_LAUNCH_NEXT((grad_sum_kernel<TG, TO, true>), (int)sum_grid, kSumWarps * 32, 0, k.st, a);
+      else HB_LAUNCH_NEXT((grad_sum_kernel<TG, TO, false>), (int)sum_grid, kSumWarps * 32, 0, k.st, a);
       return HB_OK;
     });
   });
   if (rc != HB_OK || join_grid == 0) return rc;
   return with_type(k.out_type, [&](auto to) -> int {
-    HB_LAUNCH(grad_join_kernel<decltype(to)>, (int)join_grid, kThreads, 0, k.st, a);
+    HB_LAUNCH_NEXT((grad_join_kernel<decltype(to)>), (int)join_grid, kThreads, 0, k.st, a, width, spans);
     return HB_OK;
   });
 }
