@@ -19,87 +19,23 @@ its gradient accumulation belongs to another stream, which a capture cannot wait
 """
 from __future__ import annotations
 
-import weakref
-
 import torch
 import torch.nn as nn
-from torch.utils.weak import WeakIdKeyDictionary
 
 from . import EmbCacheLib as E
-
-_GRAPHS = WeakIdKeyDictionary()  # leaf -> the live graphs of it that were built outside of a capture
-
-
-def _capturing() -> bool:
-    return torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
-
-
-def _note(ctx, leaf: torch.Tensor) -> None:
-    """Remember on a leaf which graphs of it live that were built outside of a capture; inside of one there may be none."""
-    ctx.captured = _capturing()
-    if not (leaf.requires_grad and leaf.is_leaf):
-        return
-    graphs = _GRAPHS.get(leaf)
-    if ctx.captured:
-        if graphs:
-            raise RuntimeError("Check failed: a graph of the same leaf that was built outside of this capture still lives "
-                               "(drop its outputs first)")
-        return
-    if graphs is None:
-        graphs = _GRAPHS[leaf] = weakref.WeakSet()
-    graphs.add(ctx)
-
-
-def _refuse_foreign(ctx) -> None:
-    if _capturing() and not ctx.captured:
-        raise RuntimeError("Check failed: the forward pass belongs to the capture that its backward pass is in")
-
-
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, weight, ids, scale, padding_idx, dropout, seed, offset, rng, dtype):
-        _note(ctx, weight)
-        ctx.save_for_backward(ids, rng)
-        ctx.call = (weight.size(0), scale, padding_idx, dropout, seed, offset, weight.dtype)
-        return E.cudaEmbedding(weight, ids, scale, padding_idx, dropout, seed, offset, rng, dtype)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        _refuse_foreign(ctx)
-        ids, rng = ctx.saved_tensors
-        rows, scale, padding_idx, dropout, seed, offset, dtype = ctx.call
-        return (E.cudaEmbeddingGrad(ids, grad, rows, scale, padding_idx, dropout, seed, offset, rng, dtype),
-                None, None, None, None, None, None, None, None)
-
-
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, p, seed, offset, rng, scale, dtype):
-        _note(ctx, x)
-        ctx.save_for_backward(rng)
-        ctx.call = (p, seed, offset, scale, x.dtype)
-        return E.cudaDropout(x, p, seed, offset, rng, scale, dtype)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        _refuse_foreign(ctx)
-        (rng,) = ctx.saved_tensors
-        p, seed, offset, scale, dtype = ctx.call
-        return E.cudaDropout(grad, p, seed, offset, rng, scale, dtype), None, None, None, None, None, None
+from . import _lib
 
 
 def embedding(weight, ids, scale: float = 1.0, padding_idx: int | None = None, dropout: float = 0.0, seed: int = 0,
               offset: int = 0, rng: torch.Tensor | None = None, dtype: torch.dtype | None = None) -> torch.Tensor:
-    """``cudaEmbedding``, differentiable in weight (all of whose rows the gradient has, zeros where no token points)."""
-    return _Embedding.apply(weight, ids, scale, padding_idx, dropout, seed, offset, rng, dtype)
+    """``cudaEmbedding``, differentiable (once) in weight, all of whose rows the gradient has, zeros where no token points."""
+    return (_lib._NATIVE or _lib.native()).embedding_autograd(weight, ids, scale, padding_idx, dropout, seed, offset, rng, dtype)
 
 
 def dropout(x, p: float, seed: int = 0, offset: int = 0, rng: torch.Tensor | None = None, scale: float = 1.0,
             dtype: torch.dtype | None = None) -> torch.Tensor:
-    """``cudaDropout``, differentiable in x."""
-    return _Dropout.apply(x, p, seed, offset, rng, scale, dtype)
+    """``cudaDropout``, differentiable (once) in x."""
+    return (_lib._NATIVE or _lib.native()).dropout_autograd(x, scale, p, seed, offset, rng, dtype)
 
 
 class DropoutSeeds:

@@ -344,6 +344,48 @@ def test_autograd(E):
         assert torch.equal(x.grad, E.cudaDropout(g[0, :9], 0.25, 5, 6, scale=2.0))
 
 
+def test_autograd_refusals(E):
+    from hades_b200 import token_emb
+
+    w = torch.randn(20, 16, device="cuda").requires_grad_()
+    ids = torch.arange(8, device="cuda")
+    h = token_emb.embedding(w, ids, dropout=0.5)
+    (g,) = torch.autograd.grad((h * h).sum(), w, create_graph=False)
+    h = token_emb.embedding(w, ids)
+    with pytest.raises(RuntimeError, match="not differentiated again"):
+        torch.autograd.grad((h * h).sum(), w, create_graph=True)
+    h = token_emb.embedding(w, ids)
+    assert torch.autograd.grad(h.sum(), w, create_graph=True)[0][:8].eq(1).all()  # (does not depend on anything)
+    h = token_emb.embedding(w, ids)
+    ids += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        h.sum().backward()
+    rng = torch.tensor([1, 2], device="cuda")
+    h = token_emb.dropout(w, 0.5, rng=rng)
+    rng += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        h.sum().backward()
+    h = token_emb.embedding(w, ids)
+    h.sum().backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        h.sum().backward()
+    assert not token_emb.embedding(w.detach(), ids).requires_grad
+    with torch.no_grad():
+        assert not token_emb.embedding(w, ids).requires_grad
+    # a weight that is computed, used twice
+    v = torch.randn(20, 16, device="cuda").requires_grad_()
+    u = v * 3
+    (token_emb.embedding(u, ids) + token_emb.embedding(u, ids, scale=2.0)).sum().backward()
+    want = torch.zeros_like(v)
+    want[ids] = 9.0
+    assert torch.equal(v.grad, want)
+    # an output that nothing depends on
+    x = torch.randn(4, 16, device="cuda").requires_grad_()
+    a, b = token_emb.dropout(x, 0.5, 1, 1), token_emb.dropout(x, 0.5, 1, 2)
+    a.sum().backward()
+    assert torch.equal(x.grad, E.cudaDropout(torch.ones_like(x), 0.5, 1, 1)) and b.requires_grad
+
+
 def test_gradient_against_differences(E):
     """Small whole numbers and a share of one half: every product and sum is exact, and so is the difference quotient."""
     from hades_b200 import token_emb
@@ -522,3 +564,20 @@ def test_a_capture_refuses_what_it_cannot_wait_for(E):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(kept, w.detach()[:8])
+    # any other operator's graph of the leaf is one too; two in the same capture are none
+    other = w * 2
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="still lives"):
+            token_emb.embedding(w, ids)
+        with pytest.raises(RuntimeError, match="still lives"):
+            token_emb.dropout(w, 0.5)
+        kept = E.cudaEmbedding(w.detach(), ids)
+    del other
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        w.grad = None
+        (token_emb.embedding(w, ids) + token_emb.embedding(w, ids, scale=2.0)).sum().backward()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert bool((w.grad[:8] == 3).all()) and not w.grad[8:].any()
