@@ -263,6 +263,38 @@ __device__ __forceinline__ void words_of(const float (&x)[kBlockCols], Words<blo
   }
 }
 
+// sum += value j of a word of two, or of a word of one (j = 0), in one instruction
+template <typename T>
+__device__ __forceinline__ void add_value(float& sum, uint32_t w, int j) {
+  if constexpr (sizeof(T) == 4) {
+    sum += __uint_as_float(w);
+  } else if constexpr (std::is_same_v<T, __half>) {
+    if (j == 0) asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; add.rn.f32.f16 %0, l, %0;}" : "+f"(sum) : "r"(w));
+    else asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; add.rn.f32.f16 %0, h, %0;}" : "+f"(sum) : "r"(w));
+  } else {
+    if (j == 0) asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; add.rn.f32.bf16 %0, l, %0;}" : "+f"(sum) : "r"(w));
+    else asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; add.rn.f32.bf16 %0, h, %0;}" : "+f"(sum) : "r"(w));
+  }
+}
+// Adds a block to a sum: all of it, or what is kept of it.
+template <typename T>
+__device__ __forceinline__ void add_block(float (&sum)[kBlockCols], const Words<block_words<T>()>& v) {
+  constexpr int per = 4 / (int)sizeof(T);
+#pragma unroll
+  for (int i = 0; i < kBlockCols; ++i) add_value<T>(sum[i], v.w[i / per], i % per);
+}
+template <typename T>
+__device__ __forceinline__ void add_kept(float (&sum)[kBlockCols], const Words<block_words<T>()>& v, const PhiloxKey& k,
+                                         uint32_t drop_below, uint32_t block, uint32_t row) {
+  constexpr int per = 4 / (int)sizeof(T);
+  if (drop_below > 0xffffu) return;  // none of it
+  const uint4 d = philox(make_uint4(block, row, k.offset_lo, k.offset_hi), k.k0, k.k1);
+  const uint32_t word[4] = {d.x, d.y, d.z, d.w}, top = drop_below << 16;
+#pragma unroll
+  for (int i = 0; i < kBlockCols; ++i)
+    if ((i & 1 ? word[i / 2] : word[i / 2] << 16) >= top) add_value<T>(sum[i], v.w[i / per], i % per);
+}
+
 #endif  // __CUDACC__
 
 // f(T{}) for the value type of a matrix

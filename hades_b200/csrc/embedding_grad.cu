@@ -64,14 +64,14 @@ __global__ void __launch_bounds__(kThreads) token_keys_kernel(const Id* ids, int
 
 // ---- sums ---------------------------------------------------------------------------------------------------------------
 struct Link {        // of a piece whose last token goes on behind it and does not come from before it
-  int64_t row;       // of the output
+  int64_t to;        // where its row of the output begins, in values
   int64_t pieces;    // behind this one that the token lies in; 0: no such token
 };
 
 struct GradArgs {
   hb_runs_t runs;
   const void* grads;
-  int64_t grad_stride;
+  uint32_t grad_step;            // bytes from one row to the next
   int chunk;                     // bytes of a copy: 16, 8, 4; 2: copies of 4 that may begin 2 bytes early
   uint32_t cols, blocks, tiles;  // columns, blocks of eight, tiles of `lanes` blocks
   int lanes;                     // of a unit, a power of two; a warp holds 32 / lanes units, pieces that follow one another
@@ -163,13 +163,13 @@ __device__ __forceinline__ void copied_block(const char* stage, const T* p, int 
   }
 }
 
-// WIDE: copies of 16 bytes.
+// WIDE: copies of 16 bytes, and an output whose blocks can be moved at once.
 template <typename TG, typename TO, bool WIDE>
 __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs a) {
   begin_after_previous();
   __shared__ alignas(16) char s_ring[kSumWarps][kStages][stage_bytes<TG>()];
-  __shared__ int64_t s_row[kSumWarps][kWindow];          // of the output, for every entry
-  __shared__ uint32_t s_entry[kSumWarps][kWindow + 1];   // its position; kHead: a token begins
+  __shared__ int64_t s_to[kSumWarps][kWindow];                           // where its row of the output begins, in values
+  __shared__ alignas(16) uint32_t s_entry[kSumWarps][kWindow + kStages];  // its position; kHead: a token begins
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t index = blockIdx.x * (int64_t)kSumWarps + warp;
   if (a.num_unique && blockIdx.x == 0 && threadIdx.x == 0) {  // (the run of what takes no part is the last one)
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs
       const int64_t run = a.runs.base8[j >> 3] + __popc(octet & ((2u << (lane & 7)) - 1u)) - 1;
       const int64_t token = a.runs.uniq_ids[run];
       part = token < a.num_rows;
-      if (i < length) s_row[warp][i] = a.by_run ? run : token;
+      if (i < length) s_to[warp][i] = (a.by_run ? run : token) * a.out.stride;
       s_entry[warp][i] = part ? a.runs.perm[j] | (head ? kHead : 0u) : kHead;
     } else if (i <= length) {
       s_entry[warp][i] = kHead;
@@ -215,57 +215,73 @@ __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs
   }
   const uint32_t* entry = s_entry[warp];
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_ring[warp][0]);
-  const TG* grads = static_cast<const TG*>(a.grads) + c;
+  const char* grads = static_cast<const char*>(a.grads) + c * sizeof(TG);
+  TO* const out = static_cast<TO*>(a.out.p) + c;
   const int bytes = (int)(a.cols - c) * (int)sizeof(TG);
-  auto row_of = [&](int e) { return grads + (int64_t)(entry[e] & ~kHead) * a.grad_stride; };
-  auto issue = [&](int e, int stage) {
-    if (e < to) {
-      copy_block<TG, WIDE>(ring + stage * stage_bytes<TG>(), row_of(e), a.chunk, bytes, lane);
-      if (a.out.accumulate && (entry[e] & kHead))
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<TO*>(a.out.p) + s_row[warp][e] * a.out.stride + c));
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+  auto row_of = [&](uint32_t word) {
+    return reinterpret_cast<const TG*>(grads + (uint64_t)(word & ~kHead) * a.grad_step);
   };
+  auto load_words4 = [&](int e, uint32_t (&w)[kStages]) {  // (what lies behind the unit's entries is not used)
 #pragma unroll
-  for (int s = 0; s < kStages; ++s) issue(from + s, s);
+    for (int k = 0; k < kStages; k += 4) {
+      const uint4 q = *reinterpret_cast<const uint4*>(entry + e + k);
+      w[k] = q.x; w[k + 1] = q.y; w[k + 2] = q.z; w[k + 3] = q.w;
+    }
+  };
+  uint32_t now[kStages];
+  load_words4(from, now);
+#pragma unroll
+  for (int k = 0; k < kStages; ++k) {
+    if (from + k < to) copy_block<TG, WIDE>(ring + k * stage_bytes<TG>(), row_of(now[k]), a.chunk, bytes, lane);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
   PhiloxKey key = {};
   if (a.drop.drop_below) key = philox_key(a.drop);
   float sum[kBlockCols];
 #pragma unroll
   for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
-  bool before = !(entry[from] & kHead);  // the sum belongs to a token that began before the piece
-  int stage = 0;
-  for (int e = from; e < to; ++e) {
-    if (e > from && (entry[e] & kHead)) {  // the token before ends
-      if (before) put_part(part_at(a, piece, 0, block), sum);
-      else put_row<TO>(a.out, s_row[warp][e - 1], block, sum);
+  bool before = !(now[0] & kHead);  // the sum belongs to a token that began before the piece
+  now[0] &= ~kHead;                 // (nothing ends there)
+  for (int e0 = from; e0 < to; e0 += kStages) {
+    uint32_t next[kStages];
+    load_words4(e0 + kStages < to ? e0 + kStages : e0, next);
 #pragma unroll
-      for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
-      before = false;
+    for (int k = 0; k < kStages; ++k) {
+      const int e = e0 + k;
+      if (e >= to) break;
+      if (now[k] & kHead) {  // the token before ends
+        if (before) put_part(part_at(a, piece, 0, block), sum);
+        else put_block<TO, WIDE>(a.out, out + s_to[warp][e - 1], c, sum);
+#pragma unroll
+        for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
+        before = false;
+      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      Words<block_words<TG>()> in;
+      copied_block<TG, WIDE>(s_ring[warp][k], row_of(now[k]), a.chunk, lane, in);
+      if (a.drop.drop_below) add_kept<TG>(sum, in, key, a.drop.drop_below, block, now[k] & ~kHead);
+      else add_block<TG>(sum, in);
+      if (e + kStages < to) {
+        copy_block<TG, WIDE>(ring + k * stage_bytes<TG>(), row_of(next[k]), a.chunk, bytes, lane);
+        if (a.out.accumulate && (next[k] & kHead)) asm volatile("prefetch.global.L2 [%0];" ::"l"(out + s_to[warp][e + kStages]));
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-    Words<block_words<TG>()> in;
-    copied_block<TG, WIDE>(s_ring[warp][stage], row_of(e), a.chunk, lane, in);
-    float x[kBlockCols];
-    values_of<TG>(in, x);
-    if (a.drop.drop_below) drop_block(x, key, a.drop.drop_below, 1.0f, block, entry[e] & ~kHead);
 #pragma unroll
-    for (int i = 0; i < kBlockCols; ++i) sum[i] += x[i];
-    issue(e + kStages, stage);
-    stage = stage + 1 == kStages ? 0 : stage + 1;
+    for (int k = 0; k < kStages; ++k) now[k] = next[k];
   }
   const bool ends = (entry[to] & kHead) != 0;  // the last token goes no further
   Link link{0, 0};
   if (before) {
     put_part(part_at(a, piece, 0, block), sum);
   } else if (ends) {
-    put_row<TO>(a.out, s_row[warp][to - 1], block, sum);
+    put_block<TO, WIDE>(a.out, out + s_to[warp][to - 1], c, sum);
   } else {
     put_part(part_at(a, piece, 1, block), sum);
     if (leads) {
       const int64_t behind = begin + to;  // (a multiple of 8, as the piece is full)
       const int64_t run = a.runs.base8[behind >> 3] - 1;
-      link = Link{s_row[warp][to - 1], (a.runs.run_start[run + 1] - 1) / a.per - piece};
+      link = Link{s_to[warp][to - 1], (a.runs.run_start[run + 1] - 1) / a.per - piece};
     }
   }
   if (leads) a.links[piece] = link;
@@ -305,7 +321,8 @@ __global__ void __launch_bounds__(kThreads) grad_join_kernel(const GradArgs a, i
 #pragma unroll
         for (int i = 0; i < kBlockCols; ++i) sum[i] += s_sum[w * width + threadIdx.x][i];
   }
-  if (mine == 0 && block < a.blocks) put_row<TO>(a.out, link.row, block, sum);
+  if (mine == 0 && block < a.blocks)
+    put_block<TO, false>(a.out, static_cast<TO*>(a.out.p) + link.to + block * kBlockCols, block * kBlockCols, sum);
 }
 
 struct GradPlan {
@@ -350,7 +367,7 @@ int check_call(const GradCall& k) {
   HB_CHECK_ARG(type_known(k.grad_type) && type_known(k.out_type), "%s: unknown value type", k.who);
   HB_CHECK_ARG(k.idx_bytes == 4 || k.idx_bytes == 8, "%s: idx_bytes must be 4 or 8", k.who);
   HB_CHECK_ARG(k.n == 0 || (k.ids && k.grads), "%s: null argument", k.who);
-  HB_CHECK_ARG(k.grad_stride >= 0, "%s: bad gradient stride", k.who);
+  HB_CHECK_ARG(k.grad_stride >= 0 && k.grad_stride < ((int64_t)1 << 30), "%s: bad gradient stride", k.who);
   HB_CHECK_ARG(!k.out || !overlap(k.grads, k.grad_stride, k.grad_type, k.n, k.out, k.out_stride, k.out_type,
                                   k.by_run ? k.n : k.num_rows, k.dim),
                "%s: the output lies in the gradients", k.who);
@@ -406,7 +423,7 @@ int grad(const GradCall& k) {
   if (rc != HB_OK) return rc;
   HB_CUDA(aside.join());
   a.grads = k.grads;
-  a.grad_stride = k.grad_stride;
+  a.grad_step = (uint32_t)(k.grad_stride * type_bytes(k.grad_type));
   const uint64_t ends = (uint64_t)(uintptr_t)k.grads | (uint64_t)(k.grad_stride * type_bytes(k.grad_type)) |
                         (uint64_t)(k.dim * type_bytes(k.grad_type)) | 16u;
   a.chunk = (int)(ends & (~ends + 1));
@@ -422,6 +439,8 @@ int grad(const GradCall& k) {
   a.num_rows = k.num_rows;
   a.by_run = k.by_run;
   a.num_unique = k.num_unique;
+  const bool wide = a.chunk == 16 && whole_blocks(k.out, k.out_stride, k.out_type, k.dim);
+  if (!wide && a.chunk == 16) a.chunk = 8;
   const int64_t warps = ceil_div(p.pieces, 32 / p.lanes) * p.tiles, sum_grid = ceil_div(warps, kSumWarps);
   int width = 1;
   while (width < kThreads && width < (int)p.blocks) width *= 2;
@@ -432,7 +451,7 @@ int grad(const GradCall& k) {
     return with_type(k.out_type, [&](auto to) -> int {
       using TG = decltype(tg);
       using TO = decltype(to);
-      if (a.chunk == 16) HB_LAUNCH_NEXT((grad_sum_kernel<TG, TO, true>), (int)sum_grid, kSumWarps * 32, 0, k.st, a);
+      if (wide) HB_LAUNCH_NEXT((grad_sum_kernel<TG, TO, true>), (int)sum_grid, kSumWarps * 32, 0, k.st, a);
       else HB_LAUNCH_NEXT((grad_sum_kernel<TG, TO, false>), (int)sum_grid, kSumWarps * 32, 0, k.st, a);
       return HB_OK;
     });

@@ -47,11 +47,9 @@ static inline OutRows out_rows(const GradCall& k, const Dropout& drop) {
 
 #ifdef __CUDACC__
 
-// A block of a finished sum, times the factor, rounded once.  WHOLE: its blocks can be moved at once.
-template <typename TO, bool WHOLE = false>
-__device__ __forceinline__ void put_row(const OutRows& o, int64_t row, uint32_t block, float (&x)[kBlockCols]) {
-  const uint32_t c = block * kBlockCols;
-  TO* p = static_cast<TO*>(o.p) + row * o.stride + c;
+// A block of a finished sum, from column c on, times the factor, rounded once, to p.  WHOLE: its blocks can be moved at once.
+template <typename TO, bool WHOLE>
+__device__ __forceinline__ void put_block(const OutRows& o, TO* p, uint32_t c, float (&x)[kBlockCols]) {
   Words<block_words<TO>()> w;
   if (o.accumulate) {
     float y[kBlockCols];

@@ -170,6 +170,9 @@ __global__ void __launch_bounds__(kThreads, 1) grad_few_kernel(const FewArgs a) 
   if (a.drop.drop_below) key = philox_key(a.drop);
   constexpr int kFly = sizeof(TG) == 4 || !WHOLE ? 4 : 8;  // rows on their way at once
   const int units = 32 / a.lanes, l = t & (a.lanes - 1), group = t / a.lanes, groups = kThreads / a.lanes;
+  auto row_out = [&](int run) {
+    return static_cast<TO*>(a.out.p) + (a.by_run ? (int64_t)run : (int64_t)(s_words[s_start[run]] >> kBits)) * a.out.stride;
+  };
   // the last CTAs, at most a third, have the long tokens, the others the short ones
   const int long_jobs = longs * (int)a.tiles, third = ((int)gridDim.x + 2) / 3;
   const int long_ctas = long_jobs < third ? long_jobs : third, short_ctas = gridDim.x == 1 ? 1 : (int)gridDim.x - long_ctas;
@@ -230,13 +233,10 @@ __global__ void __launch_bounds__(kThreads, 1) grad_few_kernel(const FewArgs a) 
 #pragma unroll
       for (int k = 0; k < kFly; ++k) {
         if (entry[k] < 0) break;
-        float x[kBlockCols];
-        values_of<TG>(in[k], x);
-        if (a.drop.drop_below) drop_block(x, key, a.drop.drop_below, 1.0f, block, entry[k]);
-#pragma unroll
-        for (int i = 0; i < kBlockCols; ++i) sum[i] += x[i];
+        if (a.drop.drop_below) add_kept<TG>(sum, in[k], key, a.drop.drop_below, block, entry[k]);
+        else add_block<TG>(sum, in[k]);
         if (of[k] < 0) continue;
-        put_row<TO, WHOLE>(a.out, a.by_run ? of[k] : (int64_t)(s_words[s_start[of[k]]] >> kBits), block, sum);
+        put_block<TO, WHOLE>(a.out, row_out(of[k]) + c, c, sum);
 #pragma unroll
         for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
       }
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) grad_few_kernel(const FewArgs a) 
 #pragma unroll
         for (int i = 0; i < kBlockCols; ++i) sum[i] += s_sum[other >> 5][other & 31][i];
       }
-      put_row<TO, WHOLE>(a.out, a.by_run ? the : (int64_t)(s_words[s_start[the]] >> kBits), block, sum);
+      put_block<TO, WHOLE>(a.out, row_out(the) + c, c, sum);
     }
     __syncthreads();
     job += long_ctas;

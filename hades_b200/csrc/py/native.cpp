@@ -512,10 +512,10 @@ int64_t row_stride(const at::Tensor& t) {
   }
   return rows == 1 ? t.size(k - 1) : stride;
 }
-// A matrix to read: itself, or a contiguous copy where its rows are not evenly spaced.
+// A matrix to read: itself, or a contiguous copy where its rows are not evenly spaced (or gigabytes apart).
 at::Tensor readable(const at::Tensor& t, int64_t& stride) {
   stride = row_stride(t);
-  if (stride >= 0) return t;
+  if (stride >= 0 && stride < ((int64_t)1 << 30)) return t;
   stride = t.size(t.dim() - 1);
   return t.contiguous();
 }
