@@ -103,10 +103,15 @@ __device__ __forceinline__ uint4 philox(uint4 c, uint32_t k0, uint32_t k1) {
   return c;
 }
 
+// The draws of a block of a row: column 2 j in the low half of word j, 2 j + 1 in the high one.
+__device__ __forceinline__ uint4 draws_of(const PhiloxKey& k, uint32_t block, uint32_t row) {
+  return philox(make_uint4(block, row, k.offset_lo, k.offset_hi), k.k0, k.k1);
+}
+
 // Multiplies a block by the factor; zeros where values are dropped, whatever they were.
 __device__ __forceinline__ void drop_block(float (&x)[kBlockCols], const PhiloxKey& k, uint32_t drop_below, float factor,
                                            uint32_t block, uint32_t row) {
-  const uint4 w = philox(make_uint4(block, row, k.offset_lo, k.offset_hi), k.k0, k.k1);
+  const uint4 w = draws_of(k, block, row);
   const uint32_t word[4] = {w.x, w.y, w.z, w.w};
   if (drop_below > 0xffffu) {  // all of them
 #pragma unroll
@@ -284,11 +289,10 @@ __device__ __forceinline__ void add_block(float (&sum)[kBlockCols], const Words<
   for (int i = 0; i < kBlockCols; ++i) add_value<T>(sum[i], v.w[i / per], i % per);
 }
 template <typename T>
-__device__ __forceinline__ void add_kept(float (&sum)[kBlockCols], const Words<block_words<T>()>& v, const PhiloxKey& k,
-                                         uint32_t drop_below, uint32_t block, uint32_t row) {
+__device__ __forceinline__ void add_kept(float (&sum)[kBlockCols], const Words<block_words<T>()>& v, const uint4& d,
+                                         uint32_t drop_below) {
   constexpr int per = 4 / (int)sizeof(T);
   if (drop_below > 0xffffu) return;  // none of it
-  const uint4 d = philox(make_uint4(block, row, k.offset_lo, k.offset_hi), k.k0, k.k1);
   const uint32_t word[4] = {d.x, d.y, d.z, d.w}, top = drop_below << 16;
 #pragma unroll
   for (int i = 0; i < kBlockCols; ++i)

@@ -5,8 +5,8 @@
 // token they hold: a token that is a tenth of all positions costs no warp more than another.  32 lanes take 256 columns of a
 // piece; rows come through a ring of asynchronous copies in shared memory (a lane copies and reads its own eight columns, so
 // that nothing is waited for but the copy), sums stay in registers, and a row leaves as soon as its token ends.  What of a
-// token lies in two pieces or more is left as fp32 partial rows and added up by a second launch, in the order of the pieces,
-// so that the result depends on the sizes of the call alone.
+// token lies in two pieces or more is left as fp32 partial rows, and whoever leaves the last of them adds them up, in the
+// order of the pieces, so that the bits do not depend on who that is.
 #include "aside.cuh"
 #include "embedding_grad.cuh"
 #include "runs.cuh"
@@ -17,6 +17,7 @@ int* device_error_word();  // runtime.cu
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kGroup = 16;     // pieces whose parts of a token are added up first
 constexpr int kWindow = 256;   // sorted entries of a warp
 constexpr int kStages = 8;     // rows of a warp's ring
 constexpr int kSumWarps = 4;   // of a CTA
@@ -63,11 +64,6 @@ __global__ void __launch_bounds__(kThreads) token_keys_kernel(const Id* ids, int
 }
 
 // ---- sums ---------------------------------------------------------------------------------------------------------------
-struct Link {        // of a piece whose last token goes on behind it and does not come from before it
-  int64_t to;        // where its row of the output begins, in values
-  int64_t pieces;    // behind this one that the token lies in; 0: no such token
-};
-
 struct GradArgs {
   hb_runs_t runs;
   const void* grads;
@@ -78,7 +74,7 @@ struct GradArgs {
   int per;                       // sorted entries of a piece, a multiple of 8
   int64_t pieces;
   float* parts;                  // [pieces][2][tiles * lanes * 8]: what a piece has of the token before, of the token behind
-  Link* links;                   // [pieces]
+  unsigned* arrived;             // [pieces][3][tiles] parts that are there; zero before
   Dropout drop;
   OutRows out;
   int64_t num_rows;
@@ -90,8 +86,57 @@ __device__ __forceinline__ float* part_at(const GradArgs& a, int64_t piece, int 
   return a.parts + ((piece * 2 + behind) * (int64_t)(a.tiles * a.lanes) + block) * kBlockCols;
 }
 __device__ __forceinline__ void put_part(float* p, const float (&x)[kBlockCols]) {
-  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-  *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+  __stcg(reinterpret_cast<float4*>(p), make_float4(x[0], x[1], x[2], x[3]));
+  __stcg(reinterpret_cast<float4*>(p) + 1, make_float4(x[4], x[5], x[6], x[7]));
+}
+__device__ __forceinline__ void add_part(const float* p, float (&sum)[kBlockCols]) {
+  const float4 x = __ldcg(reinterpret_cast<const float4*>(p)), y = __ldcg(reinterpret_cast<const float4*>(p) + 1);
+  sum[0] += x.x; sum[1] += x.y; sum[2] += x.z; sum[3] += x.w;
+  sum[4] += y.x; sum[5] += y.y; sum[6] += y.z; sum[7] += y.w;
+}
+
+// The first and the last entry of the token of entry j, a multiple of 8 and not its first.
+struct Extent { uint32_t first, last; };
+__device__ __forceinline__ Extent token_at(const GradArgs& a, int64_t j) {
+  const int64_t run = a.runs.base8[j >> 3] - 1;
+  return {(uint32_t)a.runs.run_start[run], (uint32_t)(a.runs.run_start[run + 1] - 1)};
+}
+
+// A unit has left its part of a token that lies in several pieces.  Where that was the last of its kGroup pieces it adds
+// those up, and where that was the last of the groups, these: true, and `sum` is the token's.  mask, leader: the unit's
+// lanes.  (What a lane reads was written by lanes of the same columns: each fences its own writes, the leader counts behind
+// all of them.)
+__device__ __forceinline__ bool last_part(const GradArgs& a, const Extent& token, int64_t piece, uint32_t block, unsigned mask,
+                                          int leader, float (&sum)[kBlockCols]) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t per = (uint32_t)a.per, tile = block / a.lanes;
+  const int64_t p0 = token.first / per, p1 = token.last / per;
+  auto arrive = [&](unsigned* count, int64_t all) {
+    __threadfence();
+    __syncwarp(mask);
+    unsigned was = 0;
+    if (lane == leader) was = atomicAdd(count, 1u);
+    was = __shfl_sync(mask, was, leader);
+    if (was + 1 != (unsigned)all) return false;
+    __threadfence();
+    return true;
+  };
+  const int64_t from = piece / kGroup * kGroup, first = p0 > from ? p0 : from;
+  const int64_t last = p1 < from + kGroup - 1 ? p1 : from + kGroup - 1;
+  if (!arrive(a.arrived + (first * 3 + (first == p0)) * a.tiles + tile, last - first + 1)) return false;
+#pragma unroll
+  for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
+#pragma unroll 8
+  for (int64_t k = first; k <= last; ++k) add_part(part_at(a, k, k == p0, block), sum);
+  const int64_t g0 = p0 / kGroup, g1 = p1 / kGroup;
+  if (g0 == g1) return true;
+  put_part(part_at(a, first, first == p0, block), sum);
+  if (!arrive(a.arrived + (p0 * 3 + 2) * a.tiles + tile, g1 - g0 + 1)) return false;
+#pragma unroll
+  for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
+#pragma unroll 8
+  for (int64_t g = g0; g <= g1; ++g) add_part(part_at(a, g == g0 ? p0 : g * kGroup, g == g0, block), sum);
+  return true;
 }
 
 // ---- a lane's block of a row through shared memory: copy i of a stage at (i * 32 + lane) * bytes ------------------------
@@ -207,12 +252,11 @@ __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs
   const int64_t piece = first * units + unit;
   const uint32_t block = (uint32_t)(index - first * a.tiles) * a.lanes + (lane & (a.lanes - 1));
   const uint32_t c = block * kBlockCols;
-  const bool leads = block == 0;  // writes the piece's link
   const int from = unit * a.per, to = from + a.per < valid ? from + a.per : valid;
-  if (from >= to || block >= a.blocks) {
-    if (leads && piece < a.pieces) a.links[piece] = Link{0, 0};
-    return;
-  }
+  if (from >= to || block >= a.blocks) return;
+  const uint32_t tile_blocks = a.blocks - (block - (lane & (a.lanes - 1)));  // from the unit's first lane on
+  const int leader = unit * a.lanes, unit_lanes = tile_blocks < (uint32_t)a.lanes ? (int)tile_blocks : a.lanes;
+  const unsigned mask = (unit_lanes == 32 ? ~0u : (1u << unit_lanes) - 1u) << leader;
   const uint32_t* entry = s_entry[warp];
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_ring[warp][0]);
   const char* grads = static_cast<const char*>(a.grads) + c * sizeof(TG);
@@ -235,12 +279,16 @@ __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs
     if (from + k < to) copy_block<TG, WIDE>(ring + k * stage_bytes<TG>(), row_of(now[k]), a.chunk, bytes, lane);
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
+  const bool leads = !(now[0] & kHead), ends = (entry[to] & kHead) != 0;  // (the last token goes no further)
+  Extent lead{}, tail{};
+  if (leads) lead = token_at(a, begin + from);
+  if (!ends) tail = token_at(a, begin + to);
   PhiloxKey key = {};
   if (a.drop.drop_below) key = philox_key(a.drop);
   float sum[kBlockCols];
 #pragma unroll
   for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
-  bool before = !(now[0] & kHead);  // the sum belongs to a token that began before the piece
+  bool before = leads;              // the sum belongs to a token that began before the piece
   now[0] &= ~kHead;                 // (nothing ends there)
   for (int e0 = from; e0 < to; e0 += kStages) {
     uint32_t next[kStages];
@@ -256,10 +304,12 @@ __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs
         for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
         before = false;
       }
+      uint4 draws = make_uint4(0u, 0u, 0u, 0u);
+      if (a.drop.drop_below) draws = draws_of(key, block, now[k] & ~kHead);  // (while the row is on its way)
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
       Words<block_words<TG>()> in;
       copied_block<TG, WIDE>(s_ring[warp][k], row_of(now[k]), a.chunk, lane, in);
-      if (a.drop.drop_below) add_kept<TG>(sum, in, key, a.drop.drop_below, block, now[k] & ~kHead);
+      if (a.drop.drop_below) add_kept<TG>(sum, in, draws, a.drop.drop_below);
       else add_block<TG>(sum, in);
       if (e + kStages < to) {
         copy_block<TG, WIDE>(ring + k * stage_bytes<TG>(), row_of(next[k]), a.chunk, bytes, lane);
@@ -270,59 +320,18 @@ __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs
 #pragma unroll
     for (int k = 0; k < kStages; ++k) now[k] = next[k];
   }
-  const bool ends = (entry[to] & kHead) != 0;  // the last token goes no further
-  Link link{0, 0};
-  if (before) {
-    put_part(part_at(a, piece, 0, block), sum);
-  } else if (ends) {
+  if (!before && ends) {
     put_block<TO, WIDE>(a.out, out + s_to[warp][to - 1], c, sum);
   } else {
-    put_part(part_at(a, piece, 1, block), sum);
-    if (leads) {
-      const int64_t behind = begin + to;  // (a multiple of 8, as the piece is full)
-      const int64_t run = a.runs.base8[behind >> 3] - 1;
-      link = Link{s_to[warp][to - 1], (a.runs.run_start[run + 1] - 1) / a.per - piece};
-    }
+    put_part(part_at(a, piece, !before, block), sum);
   }
-  if (leads) a.links[piece] = link;
-}
-
-// Tokens that begin in one piece and end in another: the parts of the pieces in order, a share of them for each of the
-// `shares` rows of threads of a CTA.
-template <typename TO>
-__global__ void __launch_bounds__(kThreads) grad_join_kernel(const GradArgs a, int width, int spans) {
-  begin_after_previous();
-  __shared__ float s_sum[kThreads][kBlockCols + 1];
-  const int64_t piece = blockIdx.x / spans;
-  const Link link = a.links[piece];
-  if (link.pieces == 0) return;
-  const uint32_t block = (uint32_t)(blockIdx.x - piece * spans) * width + threadIdx.x % width;
-  const int shares = kThreads / width, mine = threadIdx.x / width;
-  const int64_t count = link.pieces + 1, share = (count + shares - 1) / shares;
-  const int64_t from = mine * share, to = from + share < count ? from + share : count;
-  float sum[kBlockCols];
-#pragma unroll
-  for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
-  if (block < a.blocks) {
-#pragma unroll 4
-    for (int64_t k = from; k < to; ++k) {
-      const float* p = part_at(a, piece + k, k == 0, block);
-      const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 4);
-      sum[0] += x.x; sum[1] += x.y; sum[2] += x.z; sum[3] += x.w;
-      sum[4] += y.x; sum[5] += y.y; sum[6] += y.z; sum[7] += y.w;
-    }
+  // the tokens that the piece begins and ends with, where they lie in others too
+#pragma unroll 1
+  for (int which = leads ? 0 : 1; which < 2; ++which) {
+    if (which == 1 && (before || ends)) break;
+    if (last_part(a, which == 0 ? lead : tail, piece, block, mask, leader, sum))
+      put_block<TO, WIDE>(a.out, out + s_to[warp][which == 0 ? from : to - 1], c, sum);
   }
-  if (share < count) {
-#pragma unroll
-    for (int i = 0; i < kBlockCols; ++i) s_sum[threadIdx.x][i] = sum[i];
-    __syncthreads();
-    if (mine == 0)
-      for (int w = 1; w < shares && w * share < count; ++w)
-#pragma unroll
-        for (int i = 0; i < kBlockCols; ++i) sum[i] += s_sum[w * width + threadIdx.x][i];
-  }
-  if (mine == 0 && block < a.blocks)
-    put_block<TO, false>(a.out, static_cast<TO*>(a.out.p) + link.to + block * kBlockCols, block * kBlockCols, sum);
 }
 
 struct GradPlan {
@@ -331,8 +340,8 @@ struct GradPlan {
   int64_t pieces;
   int64_t* keys;
   float* parts;
-  Link* links;
-  unsigned* ticket;
+  unsigned *ticket, *arrived;
+  int64_t counts;
   void* runs_ws;
   size_t runs_bytes, total;
 };
@@ -352,7 +361,8 @@ GradPlan make_plan(void* ws, int64_t n, int64_t dim) {
   Carver cv(ws ? ws : (void*)256);
   p.keys = cv.take<int64_t>(m);
   p.parts = cv.take<float>((size_t)p.pieces * 2 * p.tiles * p.lanes * kBlockCols);
-  p.links = cv.take<Link>(p.pieces);
+  p.counts = p.pieces * 3 * p.tiles;
+  p.arrived = cv.take<unsigned>(p.counts);
   p.ticket = cv.take<unsigned>(1);
   p.runs_bytes = align_up(hb_runs_workspace_bytes(m), 256);
   p.runs_ws = cv.take<char>(p.runs_bytes);
@@ -418,7 +428,7 @@ int grad(const GradCall& k) {
   if (k.n == 0) return HB_OK;
   int bits = 1;
   while ((((int64_t)1 << bits) - 1) <= k.num_rows) ++bits;  // keys up to num_rows lie below the sort's sentinel
-  rc = runs_build(p.keys, k.n, nullptr, nullptr, 0, bits, nullptr, 0, nullptr, nullptr, k.uniq_ids, nullptr, nullptr, 0,
+  rc = runs_build(p.keys, k.n, nullptr, nullptr, 0, bits, nullptr, 0, nullptr, nullptr, k.uniq_ids, nullptr, p.arrived, p.counts,
                   p.runs_ws, p.runs_bytes, &a.runs, k.st);
   if (rc != HB_OK) return rc;
   HB_CUDA(aside.join());
@@ -434,7 +444,7 @@ int grad(const GradCall& k) {
   a.per = p.per;
   a.pieces = p.pieces;
   a.parts = p.parts;
-  a.links = p.links;
+  a.arrived = p.arrived;
   a.out = out_rows(k, a.drop);
   a.num_rows = k.num_rows;
   a.by_run = k.by_run;
@@ -442,12 +452,8 @@ int grad(const GradCall& k) {
   const bool wide = a.chunk == 16 && whole_blocks(k.out, k.out_stride, k.out_type, k.dim);
   if (!wide && a.chunk == 16) a.chunk = 8;
   const int64_t warps = ceil_div(p.pieces, 32 / p.lanes) * p.tiles, sum_grid = ceil_div(warps, kSumWarps);
-  int width = 1;
-  while (width < kThreads && width < (int)p.blocks) width *= 2;
-  const int spans = (int)ceil_div(p.blocks, width);
-  const int64_t join_grid = (p.pieces - 1) * spans;
-  HB_CHECK_ARG(sum_grid < ((int64_t)1 << 31) && join_grid < ((int64_t)1 << 31), "%s: more blocks than a launch holds", k.who);
-  rc = with_type(k.grad_type, [&](auto tg) {
+  HB_CHECK_ARG(sum_grid < ((int64_t)1 << 31), "%s: more blocks than a launch holds", k.who);
+  return with_type(k.grad_type, [&](auto tg) {
     return with_type(k.out_type, [&](auto to) -> int {
       using TG = decltype(tg);
       using TO = decltype(to);
@@ -455,11 +461,6 @@ int grad(const GradCall& k) {
       else HB_LAUNCH_NEXT((grad_sum_kernel<TG, TO, false>), (int)sum_grid, kSumWarps * 32, 0, k.st, a);
       return HB_OK;
     });
-  });
-  if (rc != HB_OK || join_grid == 0) return rc;
-  return with_type(k.out_type, [&](auto to) -> int {
-    HB_LAUNCH_NEXT((grad_join_kernel<decltype(to)>), (int)join_grid, kThreads, 0, k.st, a, width, spans);
-    return HB_OK;
   });
 }
 

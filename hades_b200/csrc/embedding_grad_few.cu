@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1) grad_few_kernel(const FewArgs a) 
 #pragma unroll
       for (int k = 0; k < kFly; ++k) {
         if (entry[k] < 0) break;
-        if (a.drop.drop_below) add_kept<TG>(sum, in[k], key, a.drop.drop_below, block, entry[k]);
+        if (a.drop.drop_below) add_kept<TG>(sum, in[k], draws_of(key, block, entry[k]), a.drop.drop_below);
         else add_block<TG>(sum, in[k]);
         if (of[k] < 0) continue;
         put_block<TO, WHOLE>(a.out, row_out(of[k]) + c, c, sum);
