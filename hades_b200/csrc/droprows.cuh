@@ -56,14 +56,15 @@ static inline bool overlap(const void* a, int64_t a_stride, int a_type, int64_t 
   return a0 < b1 && b0 < a1;
 }
 
-// Bytes that a thread can move at once of every block of a matrix: as wide as its rows' starts allow, at most a block
-// (32 of fp32, 16 of the others).
-static inline int access_bytes(const void* base, int64_t stride, int type) {
-  const uint64_t bits = (uint64_t)(uintptr_t)base | (uint64_t)(stride * type_bytes(type)) | (uint64_t)(kBlockCols * type_bytes(type));
+// Bytes that a thread can move at once of every block of a matrix: as many as its rows' starts and ends allow, at most a
+// block (32 of fp32, 16 of the others).
+static inline int access_bytes(const void* base, int64_t stride, int type, int64_t dim) {
+  const int64_t e = type_bytes(type);
+  const uint64_t bits = (uint64_t)(uintptr_t)base | (uint64_t)(stride * e) | (uint64_t)(dim * e) | (uint64_t)(kBlockCols * e);
   return (int)(bits & (~bits + 1));
 }
 static inline bool whole_blocks(const void* base, int64_t stride, int type, int64_t dim) {
-  return dim % kBlockCols == 0 && access_bytes(base, stride, type) == kBlockCols * type_bytes(type);
+  return access_bytes(base, stride, type, dim) == kBlockCols * type_bytes(type);
 }
 
 // Division of 32-bit numbers by one that a launch does not change (Granlund and Montgomery, "Division by invariant
@@ -151,40 +152,37 @@ __device__ __forceinline__ void store_block(void* p, const Words<8>& v) {
 }
 
 // Loads of what no other thread of the launch writes (an in-place call reads a value before it writes it, in one thread).
-// width: access_bytes of the matrix; cols: columns of the row from the block on, eight of a whole block.
+// width: access_bytes of the matrix; cols: columns of the row from the block on.  What lies behind the row's end is not read,
+// and undefined in `v`.
 template <typename T>
 __device__ __forceinline__ void load_words(const T* p, int width, int cols, Words<block_words<T>()>& v) {
-  constexpr int W = block_words<T>();
-  if (cols < kBlockCols) {  // the end of a row
+  constexpr int W = block_words<T>(), per = 4 / (int)sizeof(T);  // values of a word
+  const uint32_t* q = reinterpret_cast<const uint32_t*>(p);
+  if (width >= 16) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) v.w[i] = 0u;
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int i = 0; i < W; ++i)
-        if (i < cols) v.w[i] = reinterpret_cast<const uint32_t*>(p)[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < kBlockCols; ++i)
-        if (i < cols) v.w[i / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
-    }
-  } else if (width >= 16) {
-#pragma unroll
-    for (int i = 0; i < W; i += 4) {
-      const uint4 t = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i);
-      v.w[i] = t.x; v.w[i + 1] = t.y; v.w[i + 2] = t.z; v.w[i + 3] = t.w;
-    }
+    for (int i = 0; i < W; i += 4)
+      if (i == 0 || i * per < cols) {
+        const uint4 t = *reinterpret_cast<const uint4*>(q + i);
+        v.w[i] = t.x; v.w[i + 1] = t.y; v.w[i + 2] = t.z; v.w[i + 3] = t.w;
+      }
   } else if (width == 8) {
 #pragma unroll
-    for (int i = 0; i < W; i += 2) {
-      const uint2 t = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint32_t*>(p) + i);
-      v.w[i] = t.x; v.w[i + 1] = t.y;
-    }
+    for (int i = 0; i < W; i += 2)
+      if (i == 0 || i * per < cols) {
+        const uint2 t = *reinterpret_cast<const uint2*>(q + i);
+        v.w[i] = t.x; v.w[i + 1] = t.y;
+      }
   } else if (width == 4) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) v.w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    for (int i = 0; i < W; ++i)
+      if (i == 0 || i * per < cols) v.w[i] = q[i];
   } else if constexpr (sizeof(T) == 2) {
-    if ((uintptr_t)p & 2u) {  // the first value, three words, the last value
-      const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+    if (cols < kBlockCols) {
+#pragma unroll
+      for (int i = 0; i < kBlockCols; ++i)
+        if (i < cols) v.w[i / 2] = i & 1 ? v.w[i / 2] | (uint32_t)h[i] << 16 : h[i];
+    } else if ((uintptr_t)p & 2u) {  // the first value, three words, the last value
       const uint32_t* m = reinterpret_cast<const uint32_t*>(h + 1);
       const uint32_t first = h[0], m0 = m[0], m1 = m[1], m2 = m[2], last = h[7];
       v.w[0] = first | m0 << 16;
@@ -193,42 +191,32 @@ __device__ __forceinline__ void load_words(const T* p, int width, int cols, Word
       v.w[3] = m2 >> 16 | last << 16;
     } else {
 #pragma unroll
-      for (int i = 0; i < W; ++i) v.w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+      for (int i = 0; i < W; ++i) v.w[i] = q[i];
     }
   }
 }
 
 template <typename T>
 __device__ __forceinline__ void store_words(T* p, int width, int cols, const Words<block_words<T>()>& v) {
-  constexpr int W = block_words<T>();
-  if (cols < kBlockCols) {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int i = 0; i < W; ++i)
-        if (i < cols) reinterpret_cast<uint32_t*>(p)[i] = v.w[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < kBlockCols; ++i)
-        if (i < cols) reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(v.w[i / 2] >> (16 * (i & 1)));
-    }
-  } else if (width >= 16) {
+  constexpr int W = block_words<T>(), per = 4 / (int)sizeof(T);
+  uint32_t* q = reinterpret_cast<uint32_t*>(p);
+  if (width >= 16) {
 #pragma unroll
     for (int i = 0; i < W; i += 4)
-      *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(p) + i) = make_uint4(v.w[i], v.w[i + 1], v.w[i + 2], v.w[i + 3]);
+      if (i == 0 || i * per < cols) *reinterpret_cast<uint4*>(q + i) = make_uint4(v.w[i], v.w[i + 1], v.w[i + 2], v.w[i + 3]);
   } else if (width == 8) {
 #pragma unroll
     for (int i = 0; i < W; i += 2)
-      *reinterpret_cast<uint2*>(reinterpret_cast<uint32_t*>(p) + i) = make_uint2(v.w[i], v.w[i + 1]);
+      if (i == 0 || i * per < cols) *reinterpret_cast<uint2*>(q + i) = make_uint2(v.w[i], v.w[i + 1]);
   } else if (width == 4) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) reinterpret_cast<uint32_t*>(p)[i] = v.w[i];
+    for (int i = 0; i < W; ++i)
+      if (i == 0 || i * per < cols) q[i] = v.w[i];
   } else if constexpr (sizeof(T) == 2) {
     uint16_t* h = reinterpret_cast<uint16_t*>(p);
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-      h[2 * i] = (uint16_t)v.w[i];
-      h[2 * i + 1] = (uint16_t)(v.w[i] >> 16);
-    }
+    for (int i = 0; i < kBlockCols; ++i)
+      if (i < cols) h[i] = (uint16_t)(v.w[i / 2] >> (16 * (i & 1)));
   }
 }
 

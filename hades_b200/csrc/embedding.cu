@@ -93,10 +93,33 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const LookupArgs a) {
 
 __device__ __forceinline__ int staged_at(int e) { return e + (e >> 3); }
 
+// A block of 16-bit values of rows that begin at any value, to words of memory: where those begin with a block's second
+// value, its first goes with the last of the lane before, if that is of the same row.  The whole warp calls it.
+__device__ __forceinline__ void store_halves(uint16_t* p, bool valid, bool first, bool last, int cols, const Words<4>& v) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t before = __shfl_up_sync(0xffffffffu, v.w[3], 1);
+  if (!valid) return;
+  if (((uintptr_t)p & 2u) == 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (2 * i + 1 < cols) reinterpret_cast<uint32_t*>(p)[i] = v.w[i];
+      else if (2 * i < cols) p[2 * i] = (uint16_t)v.w[i];
+    }
+    return;
+  }
+  if (first || lane == 0) p[0] = (uint16_t)v.w[0];
+  else *reinterpret_cast<uint32_t*>(p - 1) = before >> 16 | v.w[0] << 16;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    if (2 * i + 2 < cols) *reinterpret_cast<uint32_t*>(p + 2 * i + 1) = __funnelshift_r(v.w[i], v.w[i + 1], 16);
+    else if (2 * i + 1 < cols) p[2 * i + 1] = (uint16_t)(v.w[i] >> 16);
+  }
+  if (cols > 7 && (last || lane == 31)) p[7] = (uint16_t)(v.w[3] >> 16);
+}
+
 template <typename TI, typename TO, int U>
 __global__ void __launch_bounds__(kThreads) ragged_kernel(const LookupArgs a) {
-  __shared__ float s_row[kThreads / 32][32 * (kBlockCols + 1)];
-  float* staged = s_row[threadIdx.x >> 5];
+  __shared__ float s_row[sizeof(TO) == 4 ? kThreads / 32 : 1][32 * (kBlockCols + 1)];
   const int lane = threadIdx.x & 31;
   uint32_t row[U], block[U];
   int64_t from[U];
@@ -116,53 +139,41 @@ __global__ void __launch_bounds__(kThreads) ragged_kernel(const LookupArgs a) {
   }
   PhiloxKey key = {};
   if (a.drop.drop_below) key = philox_key(a.drop);
-  const bool direct = !a.dst_linear || a.dst_width == kBlockCols * (int)sizeof(TO);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const bool valid = row[u] < a.n;
     const uint32_t c = block[u] * kBlockCols;
+    const int cols = a.cols - c < kBlockCols ? (int)(a.cols - c) : kBlockCols;
     const int64_t at = a.first + row[u];
     float x[kBlockCols];
 #pragma unroll
     for (int i = 0; i < kBlockCols; ++i) x[i] = 0.0f;
     if (from[u] >= 0) scaled_values<TI>(a, in[u], key, block[u], (uint32_t)at, x);
-    if (direct) {
-      if (valid) {
-        Words<block_words<TO>()> out;
-        words_of<TO>(x, out);
-        store_words(static_cast<TO*>(a.dst) + at * a.dst_stride + c, a.dst_width, a.cols - c, out);
-      }
-      continue;
-    }
-    // the warp's blocks are one stretch of memory: values [0, length) from `begin` on
-    const int mine = !valid ? 0 : a.cols - c < kBlockCols ? (int)(a.cols - c) : kBlockCols;
-    const int64_t place = at * a.cols + c;
-    const int64_t begin = __shfl_sync(0xffffffffu, place, 0);
-    const int length = __reduce_max_sync(0xffffffffu, valid ? (int)(place - begin) + mine : 0);
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < kBlockCols; ++i)
-      if (i < mine) staged[staged_at((int)(place - begin) + i)] = x[i];
-    __syncwarp();
-    TO* to = static_cast<TO*>(a.dst) + begin;
-    if constexpr (sizeof(TO) == 4) {
-      for (int e = lane; e < length; e += 32) to[e] = staged[staged_at(e)];
+    TO* to = static_cast<TO*>(a.dst) + at * a.dst_stride + c;
+    if constexpr (sizeof(TO) == 2) {
+      Words<4> out;
+      words_of<TO>(x, out);
+      if (a.dst_width == 2) store_halves(reinterpret_cast<uint16_t*>(to), valid, c == 0, c + kBlockCols >= a.cols, cols, out);
+      else if (valid) store_words(to, a.dst_width, cols, out);
+    } else if (a.dst_width > 4 || !a.dst_linear) {
+      Words<8> out;
+      words_of<TO>(x, out);
+      if (valid) store_words(to, a.dst_width, cols, out);
     } else {
-      const int odd = (int)(((uintptr_t)to >> 1) & 1u);  // words of memory begin one value earlier
-      for (int e = 2 * lane - odd; e < length; e += 64) {
-        const float lo = e >= 0 ? staged[staged_at(e)] : 0.0f, hi = e + 1 < length ? staged[staged_at(e + 1)] : 0.0f;
-        uint32_t w;
-        if constexpr (std::is_same_v<TO, __half>) {
-          const __half2 h = __floats2half2_rn(lo, hi);
-          w = *reinterpret_cast<const uint32_t*>(&h);
-        } else {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-          w = *reinterpret_cast<const uint32_t*>(&h);
-        }
-        if (e >= 0 && e + 1 < length) *reinterpret_cast<uint32_t*>(to + e) = w;
-        else if (e >= 0) *reinterpret_cast<uint16_t*>(to + e) = (uint16_t)w;
-        else *reinterpret_cast<uint16_t*>(to + e + 1) = (uint16_t)(w >> 16);
+      // single words, eight apart, would take a store eight times as long: through shared memory they leave in order (the
+      // warp's blocks are one stretch of memory: values [0, length) from `begin` on)
+      float* staged = s_row[threadIdx.x >> 5];
+      const int64_t place = at * a.cols + c;
+      const int64_t begin = __shfl_sync(0xffffffffu, place, 0);
+      const int length = __reduce_max_sync(0xffffffffu, valid ? (int)(place - begin) + cols : 0);
+      __syncwarp();
+      if (valid) {
+#pragma unroll
+        for (int i = 0; i < kBlockCols; ++i)
+          if (i < cols) staged[staged_at((int)(place - begin) + i)] = x[i];
       }
+      __syncwarp();
+      for (int e = lane; e < length; e += 32) static_cast<float*>(a.dst)[begin + e] = staged[staged_at(e)];
     }
   }
 }
@@ -173,8 +184,8 @@ int lookup(const char* who, LookupArgs a, int64_t n, int src_type, int dst_type,
   HB_CHECK_ARG(a.err != nullptr, "%s: no error word on this device", who);
   const uint32_t blocks = (a.cols + kBlockCols - 1) / kBlockCols;
   a.blocks = divisor(blocks);
-  a.src_width = access_bytes(a.src, a.src_stride, src_type);
-  a.dst_width = access_bytes(a.dst, a.dst_stride, dst_type);
+  a.src_width = access_bytes(a.src, a.src_stride, src_type, a.cols);
+  a.dst_width = access_bytes(a.dst, a.dst_stride, dst_type, a.cols);
   a.dst_linear = a.dst_stride == a.cols || n == 1;
   const bool whole = whole_blocks(a.src, a.src_stride, src_type, a.cols) && whole_blocks(a.dst, a.dst_stride, dst_type, a.cols);
   const bool few = n * blocks <= (int64_t)sm_count() * kThreads * 8;
@@ -190,7 +201,7 @@ int lookup(const char* who, LookupArgs a, int64_t n, int src_type, int dst_type,
         if (whole && few) HB_LAUNCH((rows_kernel<TI, TO, 1>), grid((int64_t)a.n * blocks, 1), kThreads, 0, st, a);
         else if (whole) HB_LAUNCH((rows_kernel<TI, TO, kRows>), grid(ceil_div(a.n, kRows) * blocks, 1), kThreads, 0, st, a);
         else if (few) HB_LAUNCH((ragged_kernel<TI, TO, 1>), grid((int64_t)a.n * blocks, 1), kThreads, 0, st, a);
-        else HB_LAUNCH((ragged_kernel<TI, TO, 2>), grid((int64_t)a.n * blocks, 2), kThreads, 0, st, a);
+        else HB_LAUNCH((ragged_kernel<TI, TO, 4>), grid((int64_t)a.n * blocks, 4), kThreads, 0, st, a);
         return HB_OK;
       });
     });

@@ -42,7 +42,7 @@ struct OutRows {
   float factor;
 };
 static inline OutRows out_rows(const GradCall& k, const Dropout& drop) {
-  return {k.out, k.out_stride, access_bytes(k.out, k.out_stride, k.out_type), (uint32_t)k.dim, k.accumulate, drop.factor};
+  return {k.out, k.out_stride, access_bytes(k.out, k.out_stride, k.out_type, k.dim), (uint32_t)k.dim, k.accumulate, drop.factor};
 }
 
 #ifdef __CUDACC__

@@ -322,7 +322,7 @@ int grad_few(const GradCall& k, const Dropout& drop, int* err) {
   f.padding = k.padding;
   f.grads = k.grads;
   f.grad_stride = k.grad_stride;
-  f.grad_width = access_bytes(k.grads, k.grad_stride, k.grad_type);
+  f.grad_width = access_bytes(k.grads, k.grad_stride, k.grad_type, k.dim);
   f.cols = (uint32_t)k.dim;
   f.blocks = (uint32_t)ceil_div(k.dim, kBlockCols);
   f.lanes = 1;
