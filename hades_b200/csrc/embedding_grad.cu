@@ -416,20 +416,24 @@ int grad(const GradCall& k) {
     z.p = nullptr;
     if (k.n == 0) return HB_OK;
   }
-  const int64_t items = z.p ? z.rows * ceil_div(z.row_bytes, z.width) : 0;
-  const int64_t key_blocks = ceil_div(k.n > items ? k.n : items, kThreads), cap = (int64_t)sm_count() * 8;
-  const int key_grid = (int)(key_blocks < cap ? key_blocks : cap);
-  if (k.idx_bytes == 8)
-    HB_LAUNCH(token_keys_kernel<int64_t>, key_grid, kThreads, 0, k.st, static_cast<const int64_t*>(k.ids), k.n, k.padding,
-              k.num_rows, p.keys, err, z);
-  else
-    HB_LAUNCH(token_keys_kernel<int32_t>, key_grid, kThreads, 0, k.st, static_cast<const int32_t*>(k.ids), k.n, k.padding,
-              k.num_rows, p.keys, err, z);
-  if (k.n == 0) return HB_OK;
   int bits = 1;
   while ((((int64_t)1 << bits) - 1) <= k.num_rows) ++bits;  // keys up to num_rows lie below the sort's sentinel
-  rc = runs_build(p.keys, k.n, nullptr, nullptr, 0, bits, nullptr, 0, nullptr, nullptr, k.uniq_ids, nullptr, p.arrived, p.counts,
-                  p.runs_ws, p.runs_bytes, &a.runs, k.st);
+  if (k.n > 0 && k.n <= kSortClusterEntries && !z.p) {
+    rc = token_runs(k, bits, p.arrived, p.counts, p.runs_ws, &a.runs);
+  } else {
+    const int64_t items = z.p ? z.rows * ceil_div(z.row_bytes, z.width) : 0;
+    const int64_t key_blocks = ceil_div(k.n > items ? k.n : items, kThreads), cap = (int64_t)sm_count() * 8;
+    const int key_grid = (int)(key_blocks < cap ? key_blocks : cap);
+    if (k.idx_bytes == 8)
+      HB_LAUNCH(token_keys_kernel<int64_t>, key_grid, kThreads, 0, k.st, static_cast<const int64_t*>(k.ids), k.n, k.padding,
+                k.num_rows, p.keys, err, z);
+    else
+      HB_LAUNCH(token_keys_kernel<int32_t>, key_grid, kThreads, 0, k.st, static_cast<const int32_t*>(k.ids), k.n, k.padding,
+                k.num_rows, p.keys, err, z);
+    if (k.n == 0) return HB_OK;
+    rc = runs_build(p.keys, k.n, nullptr, nullptr, 0, bits, nullptr, 0, nullptr, nullptr, k.uniq_ids, nullptr, p.arrived,
+                    p.counts, p.runs_ws, p.runs_bytes, &a.runs, k.st);
+  }
   if (rc != HB_OK) return rc;
   HB_CUDA(aside.join());
   a.grads = k.grads;

@@ -33,6 +33,9 @@ struct GradCall {
 bool grad_few_takes(const GradCall& k);
 int grad_few(const GradCall& k, const Dropout& drop, int* err);
 
+// Runs of the tokens in one launch (tokenruns.cu), up to kSortClusterMax of them; bits: num_rows < 2^bits.
+int token_runs(const GradCall& k, int bits, unsigned* zero, int64_t zero_words, void* workspace, hb_runs_t* out);
+
 struct OutRows {
   void* p;
   int64_t stride;

@@ -902,8 +902,9 @@ int sort_launch_grid(const Src& src, const Fin& fin, int64_t n, int max_digit, v
 
 // n: most entries the source can have; ws: sort_grid_bytes(n) bytes, 256-byte aligned (none needed for
 // n <= kSortClusterMax)
+// Up to kSortClusterMax entries.
 template <class Src, class Fin>
-int sort_run(const Src& src, const Fin& fin, int64_t n, void* ws, cudaStream_t st) {
+int sort_run_cluster(const Src& src, const Fin& fin, int64_t n, cudaStream_t st) {
   // First more CTAs, then longer chunks: what a pass issues (votes, counts, stores) is bound by one
   // SM's units, and the barrier of a larger cluster costs little more.
   if (n <= kClusterT) return sort_launch_cluster<Src, Fin, 1>(src, fin, 1, st);
@@ -917,7 +918,16 @@ int sort_run(const Src& src, const Fin& fin, int64_t n, void* ws, cudaStream_t s
   } else {
     if (n <= 32 * kClusterT) return sort_launch_cluster<Src, Fin, 2>(src, fin, 16, st);
     if (n <= 64 * kClusterT) return sort_launch_cluster<Src, Fin, 4>(src, fin, 16, st);
-    if (n <= kSortClusterMax) return sort_launch_cluster<Src, Fin, 8>(src, fin, 16, st);
+    return sort_launch_cluster<Src, Fin, 8>(src, fin, 16, st);
+  }
+}
+
+template <class Src, class Fin>
+int sort_run(const Src& src, const Fin& fin, int64_t n, void* ws, cudaStream_t st) {
+  if constexpr (Fin::kOneEach) {
+    return sort_run_cluster(src, fin, n, st);
+  } else {
+    if (n <= kSortClusterMax) return sort_run_cluster(src, fin, n, st);
     const int64_t per = ceil_div(n, sort_grid_ctas(n));
     if (per <= 2 * kGridT) return sort_launch_grid<Src, Fin, 2>(src, fin, n, kGridDigit, ws, st);
     if (per <= 4 * kGridT) return sort_launch_grid<Src, Fin, 4>(src, fin, n, kGridDigit, ws, st);
