@@ -21,14 +21,13 @@ constexpr int kGroup = 16;     // pieces whose parts of a token are added up fir
 constexpr int kWindow = 256;   // sorted entries of a warp
 constexpr int kStages = 8;     // rows of a warp's ring
 constexpr int kSumWarps = 4;   // of a CTA
-constexpr int64_t kZerosAside = 16 << 20;
 constexpr uint32_t kHead = 0x80000000u;
 
 // ---- tokens as sort keys: what takes no part (padding, ids outside of the table) sorts last, as num_rows --------------
 struct Zeros {
   char* p;          // rows to zero in the same launch, null: none
   int64_t rows, row_bytes, stride_bytes;
-  int width;        // bytes at a time: as all rows allow; of a single one 16, but for its ends
+  int width;        // bytes at a time, as all rows allow
 };
 
 template <typename Id>
@@ -42,17 +41,6 @@ __global__ void __launch_bounds__(kThreads) token_keys_kernel(const Id* ids, int
     keys[i] = inside && id != padding ? id : num_rows;
   }
   if (!z.p) return;
-  if (z.rows == 1) {
-    char *const end = z.p + z.row_bytes, *from = reinterpret_cast<char*>(((uintptr_t)z.p + 15) & ~(uintptr_t)15);
-    if (from > end) from = end;
-    char* to = from + ((end - from) & ~(int64_t)15);
-    for (char* p = from + at * 16; p < to; p += threads * 16) *reinterpret_cast<uint4*>(p) = make_uint4(0u, 0u, 0u, 0u);
-    if (at < 8) {
-      if (z.p + 2 * at < from) reinterpret_cast<uint16_t*>(z.p)[at] = 0;
-      if (to + 2 * at < end) reinterpret_cast<uint16_t*>(to)[at] = 0;
-    }
-    return;
-  }
   const int64_t per_row = z.row_bytes / z.width, items = z.rows * per_row;
   for (int64_t i = at; i < items; i += threads) {
     char* p = z.p + i / per_row * z.stride_bytes + i % per_row * z.width;
@@ -395,33 +383,31 @@ int grad(const GradCall& k) {
   }
   int* err = device_error_word();
   HB_CHECK_ARG(err != nullptr, "%s: no error word on this device", k.who);
-  Zeros z = {};
-  if (!k.by_run && !k.accumulate && k.num_rows > 0) {
-    const int64_t e = type_bytes(k.out_type);
-    z = Zeros{static_cast<char*>(k.out), k.num_rows, k.dim * e, k.out_stride * e, 0};
-    if (k.num_rows == 1 || k.out_stride == k.dim) z = Zeros{z.p, 1, k.num_rows * k.dim * e, k.num_rows * k.dim * e, 0};
-    const uint64_t bits = (uint64_t)(uintptr_t)z.p | (uint64_t)z.row_bytes | (uint64_t)z.stride_bytes | 16u;
-    z.width = z.rows == 1 ? 16 : (int)(bits & (~bits + 1));
-  }
   if (grad_few_takes(k)) return grad_few(k, a.drop, err);
   if (k.n == 0 && k.num_unique) HB_CUDA(cudaMemsetAsync(k.num_unique, 0, sizeof(int64_t), k.st));
-  if (k.n == 0 && !z.p) return HB_OK;
-  // Zeros of 16 MB and more come beside the sort, in one stretch (1.07 GB for 8,192 tokens of 4,096 bf16: 218 us with them
-  // in front of the sort, 180 beside it; below that the fork and the join cost the host as much as the zeros take).
+  // Zeros in one stretch come beside the sort (1.07 GB for 8,192 tokens of 4,096 bf16: 218 us with them in front of it, 180
+  // beside it; 8 MB 36.9 and 35.1); those of rows at a distance with the tokens' keys.
+  Zeros z = {};
   Aside aside;
-  if (z.p && z.rows == 1 && z.row_bytes >= kZerosAside) {
-    const cudaStream_t st = k.n > 0 && !stream_captures(k.st) && aside.fork(k.st) ? aside.stream() : k.st;
-    HB_CUDA(cudaMemsetAsync(p.ticket, 0, sizeof(unsigned), st));
-    HB_LAUNCH(zeros_kernel, sm_count(), 32, kZerosChunk, st, z.p, z.row_bytes, p.ticket);
-    z.p = nullptr;
-    if (k.n == 0) return HB_OK;
+  if (k.zeros()) {
+    const int64_t e = type_bytes(k.out_type);
+    if (k.num_rows == 1 || k.out_stride == k.dim) {
+      const cudaStream_t st = k.n > 0 && !stream_captures(k.st) && aside.fork(k.st) ? aside.stream() : k.st;
+      HB_CUDA(cudaMemsetAsync(p.ticket, 0, sizeof(unsigned), st));
+      HB_LAUNCH(zeros_kernel, sm_count(), 32, kZerosChunk, st, static_cast<char*>(k.out), k.num_rows * k.dim * e, p.ticket);
+    } else {
+      z = Zeros{static_cast<char*>(k.out), k.num_rows, k.dim * e, k.out_stride * e, 0};
+      const uint64_t width = (uint64_t)(uintptr_t)z.p | (uint64_t)z.row_bytes | (uint64_t)z.stride_bytes | 16u;
+      z.width = (int)(width & (~width + 1));
+    }
   }
+  if (k.n == 0 && !z.p) return HB_OK;
   int bits = 1;
   while ((((int64_t)1 << bits) - 1) <= k.num_rows) ++bits;  // keys up to num_rows lie below the sort's sentinel
   if (k.n > 0 && k.n <= kSortClusterEntries && !z.p) {
     rc = token_runs(k, bits, p.arrived, p.counts, p.runs_ws, &a.runs);
   } else {
-    const int64_t items = z.p ? z.rows * ceil_div(z.row_bytes, z.width) : 0;
+    const int64_t items = z.p ? z.rows * (z.row_bytes / z.width) : 0;
     const int64_t key_blocks = ceil_div(k.n > items ? k.n : items, kThreads), cap = (int64_t)sm_count() * 8;
     const int key_grid = (int)(key_blocks < cap ? key_blocks : cap);
     if (k.idx_bytes == 8)
