@@ -383,7 +383,7 @@ int grad(const GradCall& k) {
   }
   int* err = device_error_word();
   HB_CHECK_ARG(err != nullptr, "%s: no error word on this device", k.who);
-  if (grad_few_takes(k)) return grad_few(k, a.drop, err);
+  if (grad_few_takes(k, a.drop.drop_below > 0)) return grad_few(k, a.drop, err);
   if (k.n == 0 && k.num_unique) HB_CUDA(cudaMemsetAsync(k.num_unique, 0, sizeof(int64_t), k.st));
   // Zeros in one stretch come beside the sort (1.07 GB for 8,192 tokens of 4,096 bf16: 218 us with them in front of it, 180
   // beside it; 8 MB 36.9 and 35.1); those of rows at a distance with the tokens' keys.

@@ -30,7 +30,7 @@ struct GradCall {
 };
 
 // Few tokens, in one launch (embedding_grad_few.cu).
-bool grad_few_takes(const GradCall& k);
+bool grad_few_takes(const GradCall& k, bool dropout);
 int grad_few(const GradCall& k, const Dropout& drop, int* err);
 
 // Runs of the tokens in one launch (tokenruns.cu), up to kSortClusterMax of them; bits: num_rows < 2^bits.

@@ -31,7 +31,8 @@ struct FewArgs {
   Dropout drop;
   OutRows out;
   uint32_t num_rows;          // token and position fit in a word
-  bool by_run, zeros;
+  bool by_run, zeros, linear; // linear: a row of the output begins where the one before ends
+  Divisor row_bytes;          // of the output
   Divisor zero_pieces;        // of zero_width bytes, of a row
   int zero_width;
   int64_t stride_bytes;
@@ -276,20 +277,37 @@ __global__ void __launch_bounds__(kThreads, 1) grad_few_kernel(const FewArgs a) 
     }
     const int rows = (int)(row_end - v0 < kRows ? row_end - v0 : kRows);
     char* base = static_cast<char*>(a.out.p) + v0 * a.stride_bytes;
-    const uint32_t items = (uint32_t)rows * a.zero_pieces.by;
+    // rows that follow one another are a stretch of memory, and its pieces of 32 bytes may lie in two rows or more
+    const uint32_t skew = a.linear ? (uint32_t)((uintptr_t)base & 31u) : 0u, size = (uint32_t)rows * a.row_bytes.by;
+    const uint32_t items = a.linear ? (size + skew + 31u) / 32u : (uint32_t)rows * a.zero_pieces.by;
+    auto there = [&](uint32_t v) { return (s_there[v >> 5] >> (v & 31) & 1u) != 0u; };
     for (;;) {
       constexpr uint32_t kStretch = 256;
       uint32_t i0 = lane == 0 ? (uint32_t)atomicAdd(&s_ticket, 1) * kStretch : 0u;
       i0 = __shfl_sync(0xffffffffu, i0, 0);
       if (i0 >= items) break;
+      if (a.linear) {
+        for (uint32_t i = i0 + lane; i < i0 + kStretch && i < items; i += 32) {
+          const int from = (int)(i * 32u) - (int)skew, first = from < 0 ? 0 : from;
+          const int last = from + 31 < (int)size ? from + 31 : (int)size - 1;
+          const uint32_t v = divide(first, a.row_bytes), w = divide(last, a.row_bytes);
+          const bool none = !there(v) && !there(w);
+          if (v + 1 >= w && none && last - first == 31) {
+            store_block(base + from, Words<8>{});
+          } else if (v + 1 < w || !there(v) || !there(w)) {
+            for (int b = first; b <= last; b += (int)sizeof(TO))
+              if (!there(divide(b, a.row_bytes))) *reinterpret_cast<std::conditional_t<sizeof(TO) == 4, uint32_t, uint16_t>*>(base + b) = 0;
+          }
+        }
+        continue;
+      }
 #pragma unroll 4
       for (uint32_t i = i0 + lane; i < i0 + kStretch; i += 32) {
         if (i >= items) break;
         const uint32_t v = divide(i, a.zero_pieces);
-        if (s_there[v >> 5] >> (v & 31) & 1u) continue;
+        if (there(v)) continue;
         char* p = base + v * a.stride_bytes + (i - v * a.zero_pieces.by) * a.zero_width;
-        if (a.zero_width == 32) store_block(p, Words<8>{});
-        else if (a.zero_width == 16) *reinterpret_cast<uint4*>(p) = make_uint4(0u, 0u, 0u, 0u);
+        if (a.zero_width == 16) *reinterpret_cast<uint4*>(p) = make_uint4(0u, 0u, 0u, 0u);
         else if (a.zero_width == 8) *reinterpret_cast<uint2*>(p) = make_uint2(0u, 0u);
         else if (a.zero_width == 4) *reinterpret_cast<uint32_t*>(p) = 0u;
         else *reinterpret_cast<uint16_t*>(p) = 0;
@@ -299,19 +317,29 @@ __global__ void __launch_bounds__(kThreads, 1) grad_few_kernel(const FewArgs a) 
 }
 
 int entries_each(const GradCall& k) { return k.n <= kThreads ? 1 : k.n <= 2 * kThreads ? 2 : 4; }
-// Bytes of zeros at a time, as all rows allow.
+// Bytes of zeros at a time, as all rows at a distance allow.
 int zero_width(const GradCall& k) {
   const int64_t e = type_bytes(k.out_type);
-  const uint64_t bits = (uint64_t)(uintptr_t)k.out | (uint64_t)(k.dim * e) | (uint64_t)(k.num_rows > 1 ? k.out_stride * e : 0) | 32u;
+  const uint64_t bits = (uint64_t)(uintptr_t)k.out | (uint64_t)(k.dim * e) | (uint64_t)(k.out_stride * e) | 16u;
   return (int)(bits & (~bits + 1));
+}
+
+bool whole_rows(const GradCall& k) {
+  return whole_blocks(k.grads, k.grad_stride, k.grad_type, k.dim) && whole_blocks(k.out, k.out_stride, k.out_type, k.dim);
 }
 
 }  // namespace
 
-// Token and position in a word; pieces of kRows rows of zeros count in 32 bits.
-bool grad_few_takes(const GradCall& k) {
-  return k.n > 0 && k.n <= kMost && k.num_rows < ((int64_t)1 << 32) / (kThreads * entries_each(k)) - 1 &&
-         (!k.zeros() || k.dim * type_bytes(k.out_type) / zero_width(k) < (1 << 19));
+// Where the launches that this form spares weigh more than the sums, which the other form's ring of copies feeds better, and
+// than the zeros, which it writes beside its sort (us, this form and the other; 2,048 tokens, bf16: 4,096 columns 22.7 and
+// 24.6, 8,192 29.9 and 27.8, 4,096 with dropout 31.0 and 26.7, 4,001 53.5 and 32.1; 500 of 8,001 23.3 and 23.3; 1,024 of 4,096
+// into 131 MB 35.3 and 37.8, 262 MB 54.1 and 54.5, 1.07 GB 180 and 161).  What is held to fit: token and position a word,
+// bytes of kRows rows of zeros 31 bits.
+bool grad_few_takes(const GradCall& k, bool dropout) {
+  const int64_t row_bytes = k.dim * type_bytes(k.out_type);
+  if (k.n <= 0 || k.n > kMost || k.num_rows >= ((int64_t)1 << 32) / (kThreads * entries_each(k)) - 1) return false;
+  if (k.n * k.dim * (whole_rows(k) ? 1 : 2) * (dropout ? 2 : 1) > (8 << 20)) return false;
+  return !k.zeros() || (row_bytes < (1 << 19) && k.num_rows * row_bytes <= (192 << 20));
 }
 
 int grad_few(const GradCall& k, const Dropout& drop, int* err) {
@@ -343,11 +371,12 @@ int grad_few(const GradCall& k, const Dropout& drop, int* err) {
     f.stride_bytes = k.out_stride * type_bytes(k.out_type);
     f.zero_width = zero_width(k);
     f.zero_pieces = divisor((uint32_t)(row_bytes / f.zero_width));
+    f.row_bytes = divisor((uint32_t)row_bytes);
+    f.linear = k.num_rows == 1 || k.out_stride == k.dim;
     if (ceil_div(k.num_rows * row_bytes, 8192) > grid) grid = ceil_div(k.num_rows * row_bytes, 8192);
   }
   if (grid > sm_count()) grid = sm_count();
-  const bool whole = whole_blocks(k.grads, k.grad_stride, k.grad_type, k.dim) &&
-                     whole_blocks(k.out, k.out_stride, k.out_type, k.dim);
+  const bool whole = whole_rows(k);
   return with_type(k.grad_type, [&](auto tg) {
     return with_type(k.out_type, [&](auto to) -> int {
       using TG = decltype(tg);
