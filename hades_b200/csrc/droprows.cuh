@@ -134,7 +134,7 @@ template <int W> struct Words { uint32_t w[W]; };
 
 // Whole blocks that begin where a block can be moved at once.
 __device__ __forceinline__ void load_block(const void* p, Words<4>& v) {
-  asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+  asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]) : "l"(p));
 }
 __device__ __forceinline__ void load_block(const void* p, Words<8>& v) {
