@@ -17,9 +17,10 @@ int* device_error_word();  // runtime.cu
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kBatch = 4;      // 32 entries each, that a warp looks up at once
 constexpr int kGroup = 16;     // pieces whose parts of a token are added up first
 constexpr int kWindow = 256;   // sorted entries of a warp
-constexpr int kStages = 8;     // rows of a warp's ring
+constexpr int kStages = 4;     // rows of a warp's ring
 constexpr int kSumWarps = 4;   // of a CTA
 constexpr uint32_t kHead = 0x80000000u;
 
@@ -90,42 +91,48 @@ __device__ __forceinline__ Extent token_at(const GradArgs& a, int64_t j) {
   return {(uint32_t)a.runs.run_start[run], (uint32_t)(a.runs.run_start[run + 1] - 1)};
 }
 
-// A unit has left its part of a token that lies in several pieces.  Where that was the last of its kGroup pieces it adds
-// those up, and where that was the last of the groups, these: true, and `sum` is the token's.  mask, leader: the unit's
-// lanes.  (What a lane reads was written by lanes of the same columns: each fences its own writes, the leader counts behind
-// all of them.)
-__device__ __forceinline__ bool last_part(const GradArgs& a, const Extent& token, int64_t piece, uint32_t block, unsigned mask,
-                                          int leader, float (&sum)[kBlockCols]) {
-  const int lane = threadIdx.x & 31;
-  const uint32_t per = (uint32_t)a.per, tile = block / a.lanes;
-  const int64_t p0 = token.first / per, p1 = token.last / per;
-  auto arrive = [&](unsigned* count, int64_t all) {
+// A unit's part of a token that lies in several pieces, left in `parts`.  Whoever leaves the last one of kGroup pieces adds
+// those up, and of the groups' sums whoever leaves the last: then `sum` is the token's.
+struct Part {
+  bool on;
+  int64_t p0, p1;       // pieces that the token begins and ends in
+  int64_t first, last;  // of the unit's group
+  __device__ __forceinline__ Part(const GradArgs& a, bool on, const Extent& token, int64_t piece) : on(on) {
+    const uint32_t per = (uint32_t)a.per;
+    p0 = token.first / per;
+    p1 = token.last / per;
+    const int64_t from = piece / kGroup * kGroup;
+    first = p0 > from ? p0 : from;
+    last = p1 < from + kGroup - 1 ? p1 : from + kGroup - 1;
+  }
+  __device__ __forceinline__ unsigned* count(const GradArgs& a, uint32_t tile) const {
+    return a.arrived + (first * 3 + (first == p0)) * a.tiles + tile;
+  }
+  // was: parts of the group that were there before the unit's
+  __device__ __forceinline__ bool finish(const GradArgs& a, unsigned was, uint32_t block, unsigned mask, int leader,
+                                         float (&sum)[kBlockCols]) const {
+    if (was != (unsigned)(last - first)) return false;
+    __threadfence();
+#pragma unroll
+    for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
+#pragma unroll 8
+    for (int64_t k = first; k <= last; ++k) add_part(part_at(a, k, k == p0, block), sum);
+    const int64_t g0 = p0 / kGroup, g1 = p1 / kGroup;
+    if (g0 == g1) return true;
+    put_part(part_at(a, first, first == p0, block), sum);
     __threadfence();
     __syncwarp(mask);
-    unsigned was = 0;
-    if (lane == leader) was = atomicAdd(count, 1u);
-    was = __shfl_sync(mask, was, leader);
-    if (was + 1 != (unsigned)all) return false;
+    unsigned groups = 0;
+    if ((int)(threadIdx.x & 31) == leader) groups = atomicAdd(a.arrived + (p0 * 3 + 2) * a.tiles + block / a.lanes, 1u);
+    if (__shfl_sync(mask, groups, leader) != (unsigned)(g1 - g0)) return false;
     __threadfence();
+#pragma unroll
+    for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
+#pragma unroll 8
+    for (int64_t g = g0; g <= g1; ++g) add_part(part_at(a, g == g0 ? p0 : g * kGroup, g == g0, block), sum);
     return true;
-  };
-  const int64_t from = piece / kGroup * kGroup, first = p0 > from ? p0 : from;
-  const int64_t last = p1 < from + kGroup - 1 ? p1 : from + kGroup - 1;
-  if (!arrive(a.arrived + (first * 3 + (first == p0)) * a.tiles + tile, last - first + 1)) return false;
-#pragma unroll
-  for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
-#pragma unroll 8
-  for (int64_t k = first; k <= last; ++k) add_part(part_at(a, k, k == p0, block), sum);
-  const int64_t g0 = p0 / kGroup, g1 = p1 / kGroup;
-  if (g0 == g1) return true;
-  put_part(part_at(a, first, first == p0, block), sum);
-  if (!arrive(a.arrived + (p0 * 3 + 2) * a.tiles + tile, g1 - g0 + 1)) return false;
-#pragma unroll
-  for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
-#pragma unroll 8
-  for (int64_t g = g0; g <= g1; ++g) add_part(part_at(a, g == g0 ? p0 : g * kGroup, g == g0, block), sum);
-  return true;
-}
+  }
+};
 
 // ---- a lane's block of a row through shared memory: copy i of a stage at (i * 32 + lane) * bytes ------------------------
 template <typename T> constexpr int stage_bytes() { return 32 * (sizeof(T) == 4 ? 32 : 20); }
@@ -201,6 +208,7 @@ template <typename TG, typename TO, bool WIDE>
 __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs a) {
   begin_after_previous();
   __shared__ alignas(16) char s_ring[kSumWarps][kStages][stage_bytes<TG>()];
+  __shared__ alignas(16) char s_added[WIDE ? kSumWarps : 1][kStages][WIDE ? 32 * kBlockCols * sizeof(TO) : 16];  // rows added to
   __shared__ int64_t s_to[kSumWarps][kWindow];                           // where its row of the output begins, in values
   __shared__ alignas(16) uint32_t s_entry[kSumWarps][kWindow + kStages];  // its position; kHead: a token begins
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -216,23 +224,32 @@ __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs
   // the warp's entries, and the one behind them; entries that take no part count as heads, and lie behind all others
   const int64_t valid_entries = runs_valid_entries(a.runs);
   int valid = 0;
-  for (int i0 = 0; i0 <= length; i0 += 32) {
-    const int i = i0 + lane;
-    const int64_t j = begin + i;
-    const bool in = i <= length && j < valid_entries;
-    const bool head = in && a.runs.head[j] != 0;
-    const uint32_t octet = (__ballot_sync(0xffffffffu, head) >> (lane & ~7)) & 0xffu;
-    bool part = false;
-    if (in) {
-      const int64_t run = a.runs.base8[j >> 3] + __popc(octet & ((2u << (lane & 7)) - 1u)) - 1;
-      const int64_t token = a.runs.uniq_ids[run];
-      part = token < a.num_rows;
-      if (i < length) s_to[warp][i] = (a.by_run ? run : token) * a.out.stride;
-      s_entry[warp][i] = part ? a.runs.perm[j] | (head ? kHead : 0u) : kHead;
-    } else if (i <= length) {
-      s_entry[warp][i] = kHead;
+#pragma unroll 1
+  for (int i0 = 0; i0 <= length; i0 += 32 * kBatch) {  // (loads of a kind on their way at once)
+    uint32_t word[kBatch];
+    int64_t run[kBatch], token[kBatch];
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      const int64_t i = i0 + q * 32 + lane, j = begin + i;
+      const bool in = i <= length && j < valid_entries;
+      word[q] = in ? a.runs.perm[j] | (a.runs.head[j] ? kHead : 0u) : 0u;
+      run[q] = in ? a.runs.base8[j >> 3] - 1 : -1;
     }
-    valid += __popc(__ballot_sync(0xffffffffu, part && i < length));
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      const int64_t i = i0 + q * 32 + lane, j = begin + i;
+      const uint32_t octet = (__ballot_sync(0xffffffffu, word[q] >> 31) >> (lane & ~7)) & 0xffu;
+      run[q] += __popc(octet & ((2u << (lane & 7)) - 1u));
+      token[q] = i <= length && j < valid_entries ? a.runs.uniq_ids[run[q]] : INT64_MAX;
+    }
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      const int i = i0 + q * 32 + lane;
+      const bool part = token[q] < a.num_rows;
+      if (i <= length) s_entry[warp][i] = part ? word[q] : kHead;
+      if (i < length) s_to[warp][i] = (a.by_run ? run[q] : token[q]) * a.out.stride;
+      valid += __popc(__ballot_sync(0xffffffffu, part && i < length));
+    }
   }
   __syncwarp();
 
@@ -260,11 +277,23 @@ __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs
       w[k] = q.x; w[k + 1] = q.y; w[k + 2] = q.z; w[k + 3] = q.w;
     }
   };
+  // the row of entry e, and where a token begins with it and the sum is added to what is there, that row
+  const bool add = a.out.accumulate;
+  const uint32_t added = (uint32_t)__cvta_generic_to_shared(s_added[WIDE ? warp : 0][0]);
+  constexpr int kAddedBytes = 32 * kBlockCols * (int)sizeof(TO);
+  auto issue = [&](int e, int k, uint32_t word) {
+    copy_block<TG, WIDE>(ring + k * stage_bytes<TG>(), row_of(word), a.chunk, bytes, lane);
+    if (add && (word & kHead)) {
+      const TO* p = out + s_to[warp][e];
+      if constexpr (WIDE) copy_block<TO, true>(added + k * kAddedBytes, p, 16, kBlockCols * (int)sizeof(TO), lane);
+      else asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+    }
+  };
   uint32_t now[kStages];
   load_words4(from, now);
 #pragma unroll
   for (int k = 0; k < kStages; ++k) {
-    if (from + k < to) copy_block<TG, WIDE>(ring + k * stage_bytes<TG>(), row_of(now[k]), a.chunk, bytes, lane);
+    if (from + k < to) issue(from + k, k, now[k]);
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   const bool leads = !(now[0] & kHead), ends = (entry[to] & kHead) != 0;  // (the last token goes no further)
@@ -277,7 +306,7 @@ __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs
 #pragma unroll
   for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
   bool before = leads;              // the sum belongs to a token that began before the piece
-  now[0] &= ~kHead;                 // (nothing ends there)
+  Words<block_words<TO>()> there = {};  // of the row that the token's sum is added to
   for (int e0 = from; e0 < to; e0 += kStages) {
     uint32_t next[kStages];
     load_words4(e0 + kStages < to ? e0 + kStages : e0, next);
@@ -285,9 +314,10 @@ __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs
     for (int k = 0; k < kStages; ++k) {
       const int e = e0 + k;
       if (e >= to) break;
-      if (now[k] & kHead) {  // the token before ends
+      const bool head = (now[k] & kHead) != 0;
+      if (head && e > from) {  // the token before ends
         if (before) put_part(part_at(a, piece, 0, block), sum);
-        else put_block<TO, WIDE>(a.out, out + s_to[warp][e - 1], c, sum);
+        else put_block<TO, WIDE>(a.out, out + s_to[warp][e - 1], c, sum, WIDE ? &there : nullptr);
 #pragma unroll
         for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
         before = false;
@@ -297,27 +327,39 @@ __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
       Words<block_words<TG>()> in;
       copied_block<TG, WIDE>(s_ring[warp][k], row_of(now[k]), a.chunk, lane, in);
+      if constexpr (WIDE)
+        if (add && head) copied_block<TO, true>(s_added[warp][k], out, 16, lane, there);
       if (a.drop.drop_below) add_kept<TG>(sum, in, draws, a.drop.drop_below);
       else add_block<TG>(sum, in);
-      if (e + kStages < to) {
-        copy_block<TG, WIDE>(ring + k * stage_bytes<TG>(), row_of(next[k]), a.chunk, bytes, lane);
-        if (a.out.accumulate && (next[k] & kHead)) asm volatile("prefetch.global.L2 [%0];" ::"l"(out + s_to[warp][e + kStages]));
-      }
+      if (e + kStages < to) issue(e + kStages, k, next[k]);
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
 #pragma unroll
     for (int k = 0; k < kStages; ++k) now[k] = next[k];
   }
   if (!before && ends) {
-    put_block<TO, WIDE>(a.out, out + s_to[warp][to - 1], c, sum);
+    put_block<TO, WIDE>(a.out, out + s_to[warp][to - 1], c, sum, WIDE ? &there : nullptr);
   } else {
     put_part(part_at(a, piece, !before, block), sum);
   }
-  // the tokens that the piece begins and ends with, where they lie in others too
+  // the tokens that the piece begins and ends with, where they lie in others too.  (What a lane reads of other units was
+  // written by lanes of the same columns: each fences its own writes, and the leader counts behind all of them.)
+  const bool trails = !before && !ends;
+  if (!leads && !trails) return;
+  const Part of_lead(a, leads, lead, piece), of_tail(a, trails, tail, piece);
+  __threadfence();
+  __syncwarp(mask);
+  unsigned lead_was = 0, tail_was = 0;
+  if (lane == leader) {
+    if (leads) lead_was = atomicAdd(of_lead.count(a, block / a.lanes), 1u);
+    if (trails) tail_was = atomicAdd(of_tail.count(a, block / a.lanes), 1u);
+  }
+  lead_was = __shfl_sync(mask, lead_was, leader);
+  tail_was = __shfl_sync(mask, tail_was, leader);
 #pragma unroll 1
-  for (int which = leads ? 0 : 1; which < 2; ++which) {
-    if (which == 1 && (before || ends)) break;
-    if (last_part(a, which == 0 ? lead : tail, piece, block, mask, leader, sum))
+  for (int which = 0; which < 2; ++which) {
+    const Part& part = which == 0 ? of_lead : of_tail;
+    if (part.on && part.finish(a, which == 0 ? lead_was : tail_was, block, mask, leader, sum))
       put_block<TO, WIDE>(a.out, out + s_to[warp][which == 0 ? from : to - 1], c, sum);
   }
 }

@@ -51,12 +51,15 @@ static inline OutRows out_rows(const GradCall& k, const Dropout& drop) {
 #ifdef __CUDACC__
 
 // A block of a finished sum, from column c on, times the factor, rounded once, to p.  WHOLE: its blocks can be moved at once.
+// there: what is added to, where the caller has loaded it.
 template <typename TO, bool WHOLE>
-__device__ __forceinline__ void put_block(const OutRows& o, TO* p, uint32_t c, float (&x)[kBlockCols]) {
+__device__ __forceinline__ void put_block(const OutRows& o, TO* p, uint32_t c, float (&x)[kBlockCols],
+                                          const Words<block_words<TO>()>* there = nullptr) {
   Words<block_words<TO>()> w;
   if (o.accumulate) {
     float y[kBlockCols];
-    if constexpr (WHOLE) load_block(p, w);
+    if (there) w = *there;
+    else if constexpr (WHOLE) load_block(p, w);
     else load_words(p, o.width, o.cols - c, w);
     values_of<TO>(w, y);
 #pragma unroll
