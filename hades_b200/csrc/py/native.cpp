@@ -531,6 +531,7 @@ at::Tensor result(const at::Tensor& out, at::IntArrayRef size, at::ScalarType ty
   need(out.device() == dev && out.sizes() == size, "out has the shape of the result and lies on its device");
   stride = row_stride(out);
   need(stride >= 0, "the rows of out are contiguous and evenly spaced");
+  out.unsafeGetTensorImpl()->bump_version();  // (a graph that has saved it notices)
   return out;
 }
 

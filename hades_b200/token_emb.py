@@ -59,6 +59,15 @@ class DropoutSeeds:
         self.state[1] += 1
         return {"rng": self.state.clone()}  # (the backward pass reads it after the next call has advanced the state)
 
+    def state_dict(self) -> dict:
+        """Seed and number of masks so far, for a run that continues (one host read where they are on the GPU)."""
+        return {"seed": self.seed, "offset": self.offset if self.state is None else int(self.state[1].item())}
+
+    def load_state_dict(self, state: dict) -> None:
+        self.seed, self.offset = int(state["seed"]), int(state["offset"])
+        if self.state is not None:
+            self.state.copy_(torch.tensor([self.seed, self.offset]))
+
 
 class TokenEmbedding(nn.Module):
     """A table of [num_embeddings, embedding_dim] weights on the GPU, looked up by token.  Values are multiplied by

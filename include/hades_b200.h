@@ -793,7 +793,9 @@ int hb_step_backward(hb_step_t* s, const hb_step_desc_t* d, const int64_t* ids, 
 /* rows, python/EmbCache/dist_emb.py:199-212).                                    */
 /* Values are fp32, fp16 or bf16, in any combination of input and output; they    */
 /* are computed in fp32 and rounded once.  Strides count values from one row to   */
-/* the next; the values of a row are contiguous.                                  */
+/* the next; the values of a row are contiguous.  The first call on a device      */
+/* allocates its status word, and the first gradient of a thread a stream: make   */
+/* them outside of a stream capture.                                              */
 /* ------------------------------------------------------------------------- */
 #define HB_TYPE_F32 0
 #define HB_TYPE_F16 1
@@ -820,14 +822,14 @@ int hb_embedding(const void* weight, int weight_type, int64_t weight_stride, int
                  const hb_drop_t* drop /* nullable, host */, void* out, int out_type, int64_t out_stride,
                  hb_stream_t stream);
 
-/* y[i, :] = dropped(scale * x[i, :]); y may be x.  Its gradient is the same call on the gradient of y. */
+/* y[i, :] = dropped(scale * x[i, :]); y may be x, or else its addresses lie apart from x's.  Its gradient is the same call on the gradient of y. */
 int hb_dropout(const void* x, int x_type, int64_t x_stride, int64_t n, int64_t dim, double scale,
                const hb_drop_t* drop /* nullable, host */, void* y, int y_type, int64_t y_stride, hb_stream_t stream);
 
 /* Gradient of the table of hb_embedding from the gradients of its output: out[v, :] = scale * (sum over the positions i
  * of token v of dropped(grads[i, :])), all num_rows rows, zeros where a token does not occur; accumulate: added to what out
  * holds, rows of other tokens untouched.  Positions of padding_idx or of ids outside of the table (HB_ERR_INVALID in the
- * status word) take no part.  Sums are in fp32, in an order that depends on n and dim alone.  workspace:
+ * status word) take no part.  Sums are in fp32 and in the same order every time.  grad_stride below 2^30 values.  workspace:
  * hb_embedding_grad_workspace_bytes(n, dim), for hb_embedding_grad_rows too (0: sizes that are refused). */
 size_t hb_embedding_grad_workspace_bytes(int64_t n, int64_t dim);
 int hb_embedding_grad(const void* ids, int idx_bytes, int64_t n, int64_t padding_idx, const void* grads, int grad_type,

@@ -261,6 +261,59 @@ def test_grad_of_many_tokens(E, kind):
         check_grad(E, tokens_of(rng, kind, n, 30_000), rows_like(rng, (n, dim), BF16), 30_000, p=0.1, seed=1, offset=1)
 
 
+@pytest.mark.parametrize("n,dim,vocab,t", [(300, 1, 5000, F16), (77, 3, 700_000, F32), (500, 5, 9_001, BF16), (2048, 2, 40, F32),
+                                           (100, 1024, 60_000, F32), (2048, 4096, 30, BF16), (2000, 4001, 30, F16)])
+def test_grad_of_narrow_rows_and_large_tables(E, n, dim, vocab, t):
+    """Both forms that few tokens can take, and zeros in rows of all widths."""
+    rng = np.random.default_rng(dim)
+    ids, g = rng.integers(0, vocab, n), rows_like(rng, (n, dim), t)
+    out = torch.full((vocab, dim), math.nan, dtype=t, device="cuda")
+    E.cudaEmbeddingGrad(torch.from_numpy(ids).cuda(), g, vocab, out=out)
+    want, size, terms = oracle.embedding_grad(ids, f64(g), vocab)
+    close(out, want, t, size, terms[:, None])
+    # two rows, one of them written over by a single token, at every place of memory that rows can begin
+    for first in range(1, 9):
+        base = torch.full((3 * dim + 16,), 5.0, dtype=t, device="cuda")
+        E.cudaEmbeddingGrad(torch.ones(1, dtype=torch.int64, device="cuda"), g[:1], 3, out=base[first:first + 3 * dim].view(3, dim))
+        assert torch.equal(base[first:first + 3 * dim].view(3, dim)[1], g[0])
+        assert not base[first:first + dim].any() and not base[first + 2 * dim:first + 3 * dim].any()
+        assert bool((base[:first] == 5).all()) and bool((base[first + 3 * dim:] == 5).all())
+
+
+def test_grad_of_tokens_of_any_size(E):
+    rng = np.random.default_rng(9)
+    for n in (50, 3000):
+        ids = torch.from_numpy(rng.integers(0, 40, n) * (1 << 34) + 7).cuda()
+        g = torch.randn(n, 48, device="cuda")
+        tokens, rows = E.cudaEmbeddingGradRows(ids, g, 1 << 50, padding_idx=7)
+        small, same = E.cudaEmbeddingGradRows((ids - 7) >> 34, g, 40, padding_idx=0)
+        assert torch.equal(tokens, (small << 34) + 7)
+        # (50 tokens take two forms, which add in another order: some six terms of at most 5 each, 6 * 30 * 2^-24 = 1.1e-5)
+        torch.testing.assert_close(rows, same, rtol=0, atol=1.1e-5)
+        assert status() == 0
+        assert E.cudaEmbeddingGradRows(ids, g, 1 << 30, padding_idx=7)[0].numel() == 0 and status() == 1
+        assert E.cudaEmbeddingGrad(ids, g, 0, padding_idx=7).shape == (0, 48) and status() == 1
+
+
+@pytest.mark.parametrize("n", [700, 5000])
+@pytest.mark.parametrize("dim,first", [(64, 8), (63, 3), (100, 4), (264, 1)])
+@pytest.mark.parametrize("t", [F32, F16])
+def test_grad_added_to_rows_at_a_distance(E, n, dim, first, t):
+    rng = np.random.default_rng(n + dim)
+    ids, g = tokens_of(rng, "zipf", n, 400), rows_like(rng, (n, dim), t, 0.25)
+    base = rows_like(rng, (400, dim + 24), t)
+    start, out = base.clone(), base[:, first:first + dim]
+    E.cudaEmbeddingGrad(torch.from_numpy(ids).cuda(), g, 400, out=out, accumulate=True, dropout=0.25, seed=2, offset=3)
+    want, size, terms = oracle.embedding_grad(ids, f64(g), 400, p=0.25, seed=2, offset=3)
+    there = f64(start[:, first:first + dim])
+    close(out, want + there, t, size + np.abs(there), terms[:, None] + 1)
+    assert torch.equal(base[:, :first], start[:, :first]) and torch.equal(base[:, first + dim:], start[:, first + dim:])
+    full = torch.full_like(base, 3.0)
+    E.cudaEmbeddingGrad(torch.from_numpy(ids).cuda(), g, 400, out=full[:, first:first + dim])
+    assert torch.equal(full[:, first:first + dim], E.cudaEmbeddingGrad(torch.from_numpy(ids).cuda(), g, 400))
+    assert bool((full[:, :first] == 3).all()) and bool((full[:, first + dim:] == 3).all())
+
+
 def test_grad_of_nothing(E):
     ids, g = torch.zeros(0, dtype=torch.int64, device="cuda"), torch.zeros(0, 32, device="cuda")
     assert not E.cudaEmbeddingGrad(ids, g, 10).any()
@@ -379,6 +432,13 @@ def test_autograd_refusals(E):
     want = torch.zeros_like(v)
     want[ids] = 9.0
     assert torch.equal(v.grad, want)
+    # a tensor that a graph has saved is written over
+    y = torch.randn(8, 16, device="cuda").requires_grad_()
+    z = y * 2
+    s = (z * z).sum()
+    E.cudaEmbedding(w.detach(), ids, out=z.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        s.backward()
     # an output that nothing depends on
     x = torch.randn(4, 16, device="cuda").requires_grad_()
     a, b = token_emb.dropout(x, 0.5, 1, 1), token_emb.dropout(x, 0.5, 1, 2)
@@ -524,6 +584,33 @@ def test_captured_layer(E):
         assert torch.equal(grad, E.cudaEmbeddingGrad(ids, g, 300, 1.0, 0, 0.3, 5, offset))
         masks.append((h != 0).clone())
     assert not torch.equal(masks[0], masks[1])
+
+
+def test_captured_backward_of_many_tokens(E):
+    from hades_b200 import token_emb
+
+    w = torch.randn(900, 136, device="cuda").requires_grad_()
+    ids = torch.randint(0, 900, (5000,), device="cuda")
+    g = torch.randn(5000, 136, device="cuda")
+
+    def step():
+        w.grad = None
+        token_emb.embedding(w, ids, dropout=0.1, seed=1, offset=1).backward(g)
+        return w.grad
+
+    step()
+    torch.cuda.synchronize()
+    w.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grad = step()
+    for _ in range(2):
+        ids.copy_(torch.randint(0, 900, (5000,), device="cuda"))
+        grad.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, E.cudaEmbeddingGrad(ids, g, 900, dropout=0.1, seed=1, offset=1))
+    assert status() == 0
 
 
 def test_two_graphs_and_eager_calls_between(E):

@@ -116,6 +116,8 @@ def test_seeds():
         DropoutSeeds(-1)
     with pytest.raises(RuntimeError, match="seed"):
         DropoutSeeds(1 << 63)
+    b.load_state_dict(a.state_dict())
+    assert a.state_dict() == {"seed": 7, "offset": 2} and b.next() == a.next()
     torch.manual_seed(3)
     c = DropoutSeeds().seed
     torch.manual_seed(3)
