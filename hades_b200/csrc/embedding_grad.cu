@@ -7,6 +7,10 @@
 // that nothing is waited for but the copy), sums stay in registers, and a row leaves as soon as its token ends.  What of a
 // token lies in two pieces or more is left as fp32 partial rows, and whoever leaves the last of them adds them up, in the
 // order of the pieces, so that the bits do not depend on who that is.
+//
+// What bounds it: for many wide rows HBM, at the 5 TB/s that rows read and written all over the place reach here (65,536 x
+// 1,024 fp16 to fp32 rows: 214 MB in 42 us behind a sort of 27); for fewer the chain sort, look-up of the entries, first rows,
+// joins (8,192 x 2,048 bf16: 14 + 2 + 6 + 5 us).  With dropout the generator's 78 instructions a block come on top of some 50.
 #include "aside.cuh"
 #include "embedding_grad.cuh"
 #include "runs.cuh"
@@ -20,8 +24,11 @@ constexpr int kThreads = 256;
 constexpr int kBatch = 4;      // 32 entries each, that a warp looks up at once
 constexpr int kGroup = 16;     // pieces whose parts of a token are added up first
 constexpr int kWindow = 256;   // sorted entries of a warp
-constexpr int kStages = 4;     // rows of a warp's ring
+constexpr int kStages = 4;     // rows of a warp's ring (eight: as fast, and no room for the rows that sums are added to)
 constexpr int kSumWarps = 4;   // of a CTA
+// Warps of an SM that pieces are made for, so that all run at once (us, 65,536 x 1,024 fp16: 16 warps 69.6, 20 67.9, 24 79.7,
+// 28 75.1; two micro-batches of 16,384 x 2,048: 125.5, 121.1, 121.5, 125.8).
+constexpr int kWarpsOfSm = 20;
 constexpr uint32_t kHead = 0x80000000u;
 
 // ---- tokens as sort keys: what takes no part (padding, ids outside of the table) sorts last, as num_rows --------------
@@ -310,6 +317,7 @@ __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs
   for (int e0 = from; e0 < to; e0 += kStages) {
     uint32_t next[kStages];
     load_words4(e0 + kStages < to ? e0 + kStages : e0, next);
+    uint4 draws[2] = {};
 #pragma unroll
     for (int k = 0; k < kStages; ++k) {
       const int e = e0 + k;
@@ -322,14 +330,16 @@ __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs
         for (int i = 0; i < kBlockCols; ++i) sum[i] = 0.0f;
         before = false;
       }
-      uint4 draws = make_uint4(0u, 0u, 0u, 0u);
-      if (a.drop.drop_below) draws = draws_of(key, block, now[k] & ~kHead);  // (while the row is on its way)
+      if (k % 2 == 0 && a.drop.drop_below) {  // (of two rows at once, while they are on their way)
+        draws[0] = draws_of(key, block, now[k] & ~kHead);
+        draws[1] = draws_of(key, block, now[k + 1] & ~kHead);
+      }
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
       Words<block_words<TG>()> in;
       copied_block<TG, WIDE>(s_ring[warp][k], row_of(now[k]), a.chunk, lane, in);
       if constexpr (WIDE)
         if (add && head) copied_block<TO, true>(s_added[warp][k], out, 16, lane, there);
-      if (a.drop.drop_below) add_kept<TG>(sum, in, draws, a.drop.drop_below);
+      if (a.drop.drop_below) add_kept<TG>(sum, in, draws[k % 2], a.drop.drop_below);
       else add_block<TG>(sum, in);
       if (e + kStages < to) issue(e + kStages, k, next[k]);
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -384,7 +394,7 @@ GradPlan make_plan(void* ws, int64_t n, int64_t dim) {
   while (p.lanes < 32 && p.lanes < (int)p.blocks) p.lanes *= 2;
   p.tiles = (uint32_t)ceil_div(p.blocks, p.lanes);
   const int units = 32 / p.lanes;
-  const int64_t warps = (int64_t)sm_count() * 20;
+  const int64_t warps = (int64_t)sm_count() * kWarpsOfSm;
   const int64_t per = (int64_t)align_up((size_t)ceil_div(m * p.tiles, warps * units), 8);
   p.per = (int)(per > kWindow / units ? kWindow / units : per);
   p.pieces = ceil_div(m, p.per);

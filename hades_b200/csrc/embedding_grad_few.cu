@@ -3,8 +3,8 @@
 // Every CTA sorts all tokens for itself (bitonic, of words of token and position, so that nothing compares equal; in
 // registers, by shuffles, between warps through shared memory), and has its share of the distinct tokens, of the long ones
 // among them with all of its warps, and of the rows that no token points to.  No CTA waits for another.  Bound by latency:
-// the chain ids, sort, rows of the gradient, output; and by code that runs once and is fetched as it runs, so that long and
-// short tokens share it.
+// the chain ids, sort, rows of the gradient, output (us, 512 / 2,048 tokens: ids 1.4 / 2.3, sort 1.4 / 2.9, runs 0.9 / 1.4, rows
+// and zeros 6 / 11); and by code that runs once and is fetched as it runs, so that long and short tokens share it.
 #include <climits>
 
 #include "embedding_grad.cuh"
@@ -14,7 +14,7 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMost = 2048;
+constexpr int kMost = 2048;    // (us, 1,024 bf16 columns into 8,000 rows: 17.0, and one token more in the other form 22.6)
 constexpr int kLong = 32;      // positions of a token that a CTA adds up together
 constexpr int kRows = 4096;    // of the output, whose zeros a CTA writes at a time
 
