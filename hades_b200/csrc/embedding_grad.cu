@@ -26,9 +26,9 @@ constexpr int kGroup = 16;     // pieces whose parts of a token are added up fir
 constexpr int kWindow = 256;   // sorted entries of a warp
 constexpr int kStages = 4;     // rows of a warp's ring (eight: as fast, and no room for the rows that sums are added to)
 constexpr int kSumWarps = 4;   // of a CTA
-// Warps of an SM that pieces are made for, so that all run at once (us, 65,536 x 1,024 fp16: 16 warps 69.6, 20 67.9, 24 79.7,
-// 28 75.1; two micro-batches of 16,384 x 2,048: 125.5, 121.1, 121.5, 125.8).
-constexpr int kWarpsOfSm = 20;
+// Warps of an SM that pieces are made for, so that all run at once (us, 65,536 x 1,024 fp16: 20 warps 66.7, 24 65.3, 28 74.4;
+// 8,192 x 2,048 bf16: 30.2, 30.2, 32.8; two micro-batches of 16,384 x 2,048: 120.3, 121.4, 122.5).
+constexpr int kWarpsOfSm = 24;
 constexpr uint32_t kHead = 0x80000000u;
 
 // ---- tokens as sort keys: what takes no part (padding, ids outside of the table) sorts last, as num_rows --------------
@@ -144,6 +144,8 @@ struct Part {
 // ---- a lane's block of a row through shared memory: copy i of a stage at (i * 32 + lane) * bytes ------------------------
 template <typename T> constexpr int stage_bytes() { return 32 * (sizeof(T) == 4 ? 32 : 20); }
 
+template <typename T> constexpr int added_bytes() { return 32 * kBlockCols * (int)sizeof(T); }
+
 template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
   if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
@@ -215,7 +217,7 @@ template <typename TG, typename TO, bool WIDE>
 __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs a) {
   begin_after_previous();
   __shared__ alignas(16) char s_ring[kSumWarps][kStages][stage_bytes<TG>()];
-  __shared__ alignas(16) char s_added[WIDE ? kSumWarps : 1][kStages][WIDE ? 32 * kBlockCols * sizeof(TO) : 16];  // rows added to
+  extern __shared__ __align__(16) char s_dynamic[];  // WIDE: rows that sums are added to
   __shared__ int64_t s_to[kSumWarps][kWindow];                           // where its row of the output begins, in values
   __shared__ alignas(16) uint32_t s_entry[kSumWarps][kWindow + kStages];  // its position; kHead: a token begins
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -286,8 +288,9 @@ __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs
   };
   // the row of entry e, and where a token begins with it and the sum is added to what is there, that row
   const bool add = a.out.accumulate;
-  const uint32_t added = (uint32_t)__cvta_generic_to_shared(s_added[WIDE ? warp : 0][0]);
-  constexpr int kAddedBytes = 32 * kBlockCols * (int)sizeof(TO);
+  constexpr int kAddedBytes = added_bytes<TO>();
+  const char* s_added = s_dynamic + warp * kStages * kAddedBytes;
+  const uint32_t added = (uint32_t)__cvta_generic_to_shared(s_added);
   auto issue = [&](int e, int k, uint32_t word) {
     copy_block<TG, WIDE>(ring + k * stage_bytes<TG>(), row_of(word), a.chunk, bytes, lane);
     if (add && (word & kHead)) {
@@ -338,7 +341,7 @@ __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs
       Words<block_words<TG>()> in;
       copied_block<TG, WIDE>(s_ring[warp][k], row_of(now[k]), a.chunk, lane, in);
       if constexpr (WIDE)
-        if (add && head) copied_block<TO, true>(s_added[warp][k], out, 16, lane, there);
+        if (add && head) copied_block<TO, true>(s_added + k * kAddedBytes, out, 16, lane, there);
       if (a.drop.drop_below) add_kept<TG>(sum, in, draws[k % 2], a.drop.drop_below);
       else add_block<TG>(sum, in);
       if (e + kStages < to) issue(e + kStages, k, next[k]);
@@ -499,7 +502,8 @@ int grad(const GradCall& k) {
     return with_type(k.out_type, [&](auto to) -> int {
       using TG = decltype(tg);
       using TO = decltype(to);
-      if (wide) HB_LAUNCH_NEXT((grad_sum_kernel<TG, TO, true>), (int)sum_grid, kSumWarps * 32, 0, k.st, a);
+      const size_t added = k.accumulate ? (size_t)kSumWarps * kStages * added_bytes<TO>() : 0;
+      if (wide) HB_LAUNCH_NEXT((grad_sum_kernel<TG, TO, true>), (int)sum_grid, kSumWarps * 32, added, k.st, a);
       else HB_LAUNCH_NEXT((grad_sum_kernel<TG, TO, false>), (int)sum_grid, kSumWarps * 32, 0, k.st, a);
       return HB_OK;
     });
