@@ -189,6 +189,20 @@ def test_dropout_in_place_and_of_other_shapes(E):
     assert E.cudaDropout(x, 0.3, 5, 6, dtype=F32).dtype == F32
 
 
+def test_more_rows_than_a_launch_counts(E):
+    n = (1 << 31) + 1001  # blocks of one launch count in 31 bits, rows of a mask in 32
+    if torch.cuda.mem_get_info()[0] < 3 * 16 * n:
+        pytest.skip("needs some 100 GB")
+    x = torch.ones((n, 8), dtype=BF16, device="cuda")
+    E.cudaDropout(x, 0.5, 3, 4, out=x)
+    for row in (0, 5, (1 << 31) - 1, 1 << 31, n - 1):
+        words = oracle.philox4x32((0, row, 4, 0), (3, 0))
+        draws = np.array([int(w) >> s & 0xFFFF for w in words for s in (0, 16)])
+        assert np.array_equal(f64(x[row]), np.where(draws >= 32768, 2.0, 0.0))
+    del x
+    torch.cuda.empty_cache()
+
+
 def test_numbers_on_the_device(E):
     x = torch.randn(100, 64, device="cuda")
     for seed, offset in ((1, 2), (-1, -2), (1 << 62, 1 << 40)):
@@ -422,6 +436,11 @@ def test_autograd_refusals(E):
     h.sum().backward()
     with pytest.raises(RuntimeError, match="second time"):
         h.sum().backward()
+    w.grad = None
+    h = token_emb.embedding(w, ids)
+    h.sum().backward(retain_graph=True)
+    h.sum().backward()
+    assert bool((w.grad[ids] == 2).all())
     assert not token_emb.embedding(w.detach(), ids).requires_grad
     with torch.no_grad():
         assert not token_emb.embedding(w, ids).requires_grad
@@ -553,6 +572,32 @@ def test_another_stream(E):
     torch.cuda.synchronize()
     for k, a, b in zip((1, 2, 4), ours, theirs):
         assert torch.equal(a, want * k) and torch.equal(b, want * k)
+
+
+def test_two_threads(E):
+    import threading
+
+    ids = [torch.randint(0, 4000, (n,), device="cuda") for n in (9000, 300)]
+    grads = [torch.randn(n, 72, device="cuda") for n in (9000, 300)]
+    want = [E.cudaEmbeddingGrad(i, g, 4000, dropout=0.2, seed=1) for i, g in zip(ids, grads)]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(k):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(30):
+                got = E.cudaEmbeddingGrad(ids[k], grads[k], 4000, dropout=0.2, seed=1)
+                tokens, rows = E.cudaEmbeddingGradRows(ids[k], grads[k], 4000, dropout=0.2, seed=1)
+                if not (torch.equal(got, want[k]) and torch.equal(rows, want[k][tokens])):
+                    failed.append(k)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in (0, 1, 0, 1)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not failed and status() == 0
 
 
 def test_captured_layer(E):
