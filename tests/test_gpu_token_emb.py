@@ -257,6 +257,13 @@ def test_grad(E, kind, n, dim, vocab):
     check_grad(E, tokens_of(rng, kind, n, vocab), rows_like(rng, (n, dim), F32), vocab, scale=3.0)
 
 
+@pytest.mark.parametrize("times", [2, 8, 15, 16, 17, 32, 33, 300, 1000])
+def test_grad_of_tokens_that_repeat(E, times):
+    rng = np.random.default_rng(times)
+    for n, dim in ((1900, 136), (1000, 72), (500, 1000), (3000, 300)):
+        check_grad(E, rng.permutation(n) // times, rows_like(rng, (n, dim), BF16), n, scale=0.5)
+
+
 @pytest.mark.parametrize("gt,ot", [(F32, BF16), (F16, F32), (F16, F16), (BF16, F32), (BF16, BF16)])
 @pytest.mark.parametrize("n,dim", [(3, 17), (700, 320), (1500, 1002)])
 def test_grad_of_types_with_dropout_and_padding(E, n, dim, gt, ot):
