@@ -5,9 +5,9 @@
 // values are dropped, and what is kept is multiplied by 65536 / (65536 - T).  The generator is Philox4x32 with ten rounds
 // (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011): counter (column / 8, row, offset's
 // low and high word), key the seed.  A call's 128 bits are the draws of eight neighbouring columns, so that a place needs
-// no state and no mask in memory, forward and backward passes agree whatever kernel or layout they use, and the ten rounds
-// (some 60 instructions) cost a value 8; with 32 bits a value they would cost 15, which is more than the memory that a
-// bf16 value crosses takes.
+// no state and no mask in memory, and forward and backward passes agree whatever kernel or layout they use.  Ten rounds and
+// the eight selections are 78 of the 138 instructions that a block of bf16 values takes (65,536 x 4,096: 159 us without, 180
+// with dropout, at 62 % of the ALU's and of the wide multipliers' cycles); 32 bits a value would need twice the rounds.
 #pragma once
 
 #include <cuda_bf16.h>

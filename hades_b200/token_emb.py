@@ -71,7 +71,8 @@ class DropoutSeeds:
 
 class TokenEmbedding(nn.Module):
     """A table of [num_embeddings, embedding_dim] weights on the GPU, looked up by token.  Values are multiplied by
-    ``scale``; in training a share ``dropout`` of them is dropped."""
+    ``scale``; in training a share ``dropout`` of them is dropped.  Every forward pass draws another mask, one that is
+    computed again for a backward pass (activation checkpointing) too: call ``embedding`` with numbers of your own there."""
 
     def __init__(self, num_embeddings: int, embedding_dim: int, scale: float = 1.0, padding_idx: int | None = None,
                  dropout: float = 0.0, dtype=torch.float32, device="cuda", init_sigma: float = 0.02, seed: int | None = None,

@@ -125,11 +125,14 @@ def test_seeds():
 
 
 def test_layers_refuse_shares_outside_of_one():
+    from hades_b200.dist_emb import DistEmb
     from hades_b200.token_emb import TokenEmbedding
 
     for p in (-0.1, 1.1, math.nan):
         with pytest.raises(RuntimeError, match="dropout"):
             TokenEmbedding(4, 8, dropout=p, device="cpu")
+        with pytest.raises(RuntimeError, match="dropout"):
+            DistEmb(None, dropout=p)
 
 
 def test_oracle_gradient_is_that_of_its_forward():
