@@ -441,15 +441,20 @@ int grad(const GradCall& k) {
   if (grad_few_takes(k, a.drop.drop_below > 0)) return grad_few(k, a.drop, err);
   if (k.n == 0 && k.num_unique) HB_CUDA(cudaMemsetAsync(k.num_unique, 0, sizeof(int64_t), k.st));
   // Zeros in one stretch come beside the sort (1.07 GB for 8,192 tokens of 4,096 bf16: 218 us with them in front of it, 180
-  // beside it; 8 MB 36.9 and 35.1); those of rows at a distance with the tokens' keys.
+  // beside it; 8 MB 36.9 and 35.1), but for many beside a sort of the whole GPU: they would all leave from the few SMs that it
+  // has not taken (262,144 tokens of 1,024 into 537 MB: 424 us beside it, 267 in front; 70,000 of 1,001 into 100 MB 141 and
+  // 143, 100,000 of 256 into 26 MB 65 and 77).  Those of rows at a distance come with the tokens' keys.
   Zeros z = {};
   Aside aside;
   if (k.zeros()) {
     const int64_t e = type_bytes(k.out_type);
     if (k.num_rows == 1 || k.out_stride == k.dim) {
-      const cudaStream_t st = k.n > 0 && !stream_captures(k.st) && aside.fork(k.st) ? aside.stream() : k.st;
+      const int64_t bytes = k.num_rows * k.dim * e;
+      const bool beside = k.n > 0 && (k.n <= kSortClusterEntries || bytes <= (100 << 20)) && !stream_captures(k.st) &&
+                          aside.fork(k.st);
+      const cudaStream_t st = beside ? aside.stream() : k.st;
       HB_CUDA(cudaMemsetAsync(p.ticket, 0, sizeof(unsigned), st));
-      HB_LAUNCH(zeros_kernel, sm_count(), 32, kZerosChunk, st, static_cast<char*>(k.out), k.num_rows * k.dim * e, p.ticket);
+      HB_LAUNCH(zeros_kernel, sm_count(), 32, kZerosChunk, st, static_cast<char*>(k.out), bytes, p.ticket);
     } else {
       z = Zeros{static_cast<char*>(k.out), k.num_rows, k.dim * e, k.out_stride * e, 0};
       const uint64_t width = (uint64_t)(uintptr_t)z.p | (uint64_t)z.row_bytes | (uint64_t)z.stride_bytes | 16u;
