@@ -3,8 +3,8 @@
 //
 // The tokens are sorted with their positions (runs.cu), and the sorted entries are cut into pieces of equal length, whatever
 // token they hold: a token that is a tenth of all positions costs no warp more than another.  32 lanes take 256 columns of a
-// piece; rows come through a ring of asynchronous copies in shared memory (a lane copies and reads its own eight columns, so
-// that nothing is waited for but the copy), sums stay in registers, and a row leaves as soon as its token ends.  What of a
+// piece; rows come through a ring of asynchronous copies in shared memory (where rows begin at 16 bytes a lane copies and reads
+// its own eight columns, so that nothing is waited for but the copy), sums stay in registers, and a row leaves as soon as its token ends.  What of a
 // token lies in two pieces or more is left as fp32 partial rows, and whoever leaves the last of them adds them up, in the
 // order of the pieces, so that the bits do not depend on who that is.
 //
@@ -64,7 +64,7 @@ struct GradArgs {
   hb_runs_t runs;
   const void* grads;
   uint32_t grad_step;            // bytes from one row to the next
-  int chunk;                     // bytes of a copy: 16, 8, 4; 2: copies of 4 that may begin 2 bytes early
+  int align;                     // of the rows' starts, at most 16
   uint32_t cols, blocks, tiles;  // columns, blocks of eight, tiles of `lanes` blocks
   int lanes;                     // of a unit, a power of two; a warp holds 32 / lanes units, pieces that follow one another
   int per;                       // sorted entries of a piece, a multiple of 8
@@ -141,82 +141,70 @@ struct Part {
   }
 };
 
-// ---- a lane's block of a row through shared memory: copy i of a stage at (i * 32 + lane) * bytes ------------------------
-template <typename T> constexpr int stage_bytes() { return 32 * (sizeof(T) == 4 ? 32 : 20); }
-
+// ---- a unit's columns of a row through shared memory ----------------------------------------------------------------------
+// WIDE: rows begin at 16 bytes; a lane copies and reads its own block, copy i of a stage at (i * 32 + lane) * 16.  Others: the
+// unit copies the aligned 16 bytes that its columns lie in, as they are in memory, and a lane reads its block from where it is.
+template <typename T, bool WIDE>
+constexpr int stage_bytes() { return 32 * kBlockCols * (int)sizeof(T) + (WIDE ? 0 : 32 * 16); }
 template <typename T> constexpr int added_bytes() { return 32 * kBlockCols * (int)sizeof(T); }
 
-template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
-  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
-__device__ __forceinline__ void copy_async_part(uint32_t to, const void* from, int bytes) {  // the rest of 4: zeros
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+__device__ __forceinline__ void copy_async_part(uint32_t to, const void* from, int bytes) {  // the rest of 16: zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 
-// bytes: of the row from p on (a multiple of the chunk, whatever it is)
-template <typename T, bool WIDE>
-__device__ __forceinline__ void copy_block(uint32_t stage, const T* p, int chunk, int bytes, int lane) {
-  constexpr int B = kBlockCols * (int)sizeof(T);
-  const char* from = reinterpret_cast<const char*>(p);
-  if (WIDE) {
+template <typename T>
+__device__ __forceinline__ void copy_block(uint32_t stage, const T* p, int lane) {
 #pragma unroll
-    for (int i = 0; i < B / 16; ++i)
-      if (i == 0 || i * 16 < bytes) copy_async<16>(stage + (i * 32 + lane) * 16, from + i * 16);
-  } else if (chunk == 8) {
+  for (int i = 0; i < block_words<T>() / 4; ++i) copy_async(stage + (i * 32 + lane) * 16, reinterpret_cast<const char*>(p) + i * 16);
+}
+template <typename T>
+__device__ __forceinline__ void copied_block(const char* stage, int lane, Words<block_words<T>()>& v) {
 #pragma unroll
-    for (int i = 0; i < B / 8; ++i)
-      if (i * 8 < bytes) copy_async<8>(stage + (i * 32 + lane) * 8, from + i * 8);
-  } else if (chunk == 4) {
-#pragma unroll
-    for (int i = 0; i < B / 4; ++i)
-      if (i * 4 < bytes) copy_async<4>(stage + (i * 32 + lane) * 4, from + i * 4);
-  } else if constexpr (sizeof(T) == 2) {
-    // words of memory, the first of which may begin with the value before (of the row before, or, as an allocation
-    // begins at a word, at least of the same allocation); the last is cut where the row ends
-    const int early = (int)((uintptr_t)p & 2u);
-    const int all = early + (bytes < B ? bytes : B);
-#pragma unroll
-    for (int i = 0; i < 5; ++i)
-      if (i * 4 < all) copy_async_part(stage + (i * 32 + lane) * 4, from - early + i * 4, all - i * 4 < 4 ? all - i * 4 : 4);
+  for (int i = 0; i < block_words<T>() / 4; ++i) {
+    const uint4 t = reinterpret_cast<const uint4*>(stage)[i * 32 + lane];
+    v.w[4 * i] = t.x; v.w[4 * i + 1] = t.y; v.w[4 * i + 2] = t.z; v.w[4 * i + 3] = t.w;
   }
 }
 
-template <typename T, bool WIDE>
-__device__ __forceinline__ void copied_block(const char* stage, const T* p, int chunk, int lane, Words<block_words<T>()>& v) {
+// bytes: of the unit's columns, which begin at p; lane l of `lanes`.  (The first 16 may begin in the row before, or, as an
+// allocation begins at 16 bytes, at least in the same allocation; the last are cut where the columns end.)
+__device__ __forceinline__ void copy_span(uint32_t stage, const char* p, int bytes, int l, int lanes) {
+  const int skew = (int)((uintptr_t)p & 15u), all = skew + bytes;
+  for (int at = l * 16; at < all; at += lanes * 16) copy_async_part(stage + at, p - skew + at, all - at < 16 ? all - at : 16);
+}
+// align: of the rows' starts
+template <typename T>
+__device__ __forceinline__ void span_block(const char* stage, const char* p, int align, int l, Words<block_words<T>()>& v) {
   constexpr int W = block_words<T>();
-  if (WIDE) {
+  const int at = (int)((uintptr_t)p & 15u) + l * (kBlockCols * (int)sizeof(T));
+  if (align >= 8) {
+    const uint2* s = reinterpret_cast<const uint2*>(stage + at);
 #pragma unroll
-    for (int i = 0; i < W / 4; ++i) {
-      const uint4 t = reinterpret_cast<const uint4*>(stage)[i * 32 + lane];
-      v.w[4 * i] = t.x; v.w[4 * i + 1] = t.y; v.w[4 * i + 2] = t.z; v.w[4 * i + 3] = t.w;
+    for (int i = 0; i < W; i += 2) {
+      const uint2 t = s[i / 2];
+      v.w[i] = t.x; v.w[i + 1] = t.y;
     }
-  } else if (chunk == 8) {
-#pragma unroll
-    for (int i = 0; i < W / 2; ++i) {
-      const uint2 t = reinterpret_cast<const uint2*>(stage)[i * 32 + lane];
-      v.w[2 * i] = t.x; v.w[2 * i + 1] = t.y;
-    }
-  } else {
-    const uint32_t* s = reinterpret_cast<const uint32_t*>(stage);
-#pragma unroll
-    for (int i = 0; i < W; ++i) v.w[i] = s[i * 32 + lane];
-    if constexpr (sizeof(T) == 2) {
-      if (chunk == 2 && ((uintptr_t)p & 2u)) {
-        const uint32_t last = s[4 * 32 + lane];
-#pragma unroll
-        for (int i = 0; i < W; ++i) v.w[i] = __funnelshift_r(v.w[i], i + 1 < W ? v.w[i + 1] : last, 16);
-      }
-    }
+    return;
   }
+  const uint32_t* s = reinterpret_cast<const uint32_t*>(stage + (at & ~3));
+#pragma unroll
+  for (int i = 0; i < W; ++i) v.w[i] = s[i];
+  if constexpr (sizeof(T) == 2)
+    if (at & 2) {
+      const uint32_t last = s[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) v.w[i] = __funnelshift_r(v.w[i], i + 1 < W ? v.w[i + 1] : last, 16);
+    }
 }
 
-// WIDE: copies of 16 bytes, and an output whose blocks can be moved at once.
+// WIDE: blocks of the gradients and of the output can be moved at once.
 template <typename TG, typename TO, bool WIDE>
 __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs a) {
   begin_after_previous();
-  __shared__ alignas(16) char s_ring[kSumWarps][kStages][stage_bytes<TG>()];
+  __shared__ alignas(16) char s_ring[kSumWarps][kStages][stage_bytes<TG, WIDE>()];
   extern __shared__ __align__(16) char s_dynamic[];  // WIDE: rows that sums are added to
   __shared__ int64_t s_to[kSumWarps][kWindow];                           // where its row of the output begins, in values
   __shared__ alignas(16) uint32_t s_entry[kSumWarps][kWindow + kStages];  // its position; kHead: a token begins
@@ -272,13 +260,17 @@ __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs
   const int leader = unit * a.lanes, unit_lanes = tile_blocks < (uint32_t)a.lanes ? (int)tile_blocks : a.lanes;
   const unsigned mask = (unit_lanes == 32 ? ~0u : (1u << unit_lanes) - 1u) << leader;
   const uint32_t* entry = s_entry[warp];
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_ring[warp][0]);
-  const char* grads = static_cast<const char*>(a.grads) + c * sizeof(TG);
+  constexpr int kStageBytes = stage_bytes<TG, WIDE>();
+  const int l = lane & (a.lanes - 1);
+  const int span_at = WIDE ? 0 : unit * (a.lanes * kBlockCols * (int)sizeof(TG) + 16);  // of the unit in a stage
+  const char* stages = s_ring[warp][0] + span_at;
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(stages);
+  const uint32_t c0 = WIDE ? c : c - l * kBlockCols;  // the first column that the copies are about
+  const char* grads = static_cast<const char*>(a.grads) + c0 * sizeof(TG);
   TO* const out = static_cast<TO*>(a.out.p) + c;
-  const int bytes = (int)(a.cols - c) * (int)sizeof(TG);
-  auto row_of = [&](uint32_t word) {
-    return reinterpret_cast<const TG*>(grads + (uint64_t)(word & ~kHead) * a.grad_step);
-  };
+  const int span_cols = a.cols - c0 < (uint32_t)(a.lanes * kBlockCols) ? (int)(a.cols - c0) : a.lanes * kBlockCols;
+  const int span_bytes = span_cols * (int)sizeof(TG);
+  auto row_of = [&](uint32_t word) { return grads + (uint64_t)(word & ~kHead) * a.grad_step; };
   auto load_words4 = [&](int e, uint32_t (&w)[kStages]) {  // (what lies behind the unit's entries is not used)
 #pragma unroll
     for (int k = 0; k < kStages; k += 4) {
@@ -292,10 +284,11 @@ __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs
   const char* s_added = s_dynamic + warp * kStages * kAddedBytes;
   const uint32_t added = (uint32_t)__cvta_generic_to_shared(s_added);
   auto issue = [&](int e, int k, uint32_t word) {
-    copy_block<TG, WIDE>(ring + k * stage_bytes<TG>(), row_of(word), a.chunk, bytes, lane);
+    if constexpr (WIDE) copy_block(ring + k * kStageBytes, reinterpret_cast<const TG*>(row_of(word)), lane);
+    else copy_span(ring + k * kStageBytes, row_of(word), span_bytes, l, unit_lanes);
     if (add && (word & kHead)) {
       const TO* p = out + s_to[warp][e];
-      if constexpr (WIDE) copy_block<TO, true>(added + k * kAddedBytes, p, 16, kBlockCols * (int)sizeof(TO), lane);
+      if constexpr (WIDE) copy_block(added + k * kAddedBytes, p, lane);
       else asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
     }
   };
@@ -339,9 +332,14 @@ __global__ void __launch_bounds__(kSumWarps * 32) grad_sum_kernel(const GradArgs
       }
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
       Words<block_words<TG>()> in;
-      copied_block<TG, WIDE>(s_ring[warp][k], row_of(now[k]), a.chunk, lane, in);
-      if constexpr (WIDE)
-        if (add && head) copied_block<TO, true>(s_added + k * kAddedBytes, out, 16, lane, there);
+      if constexpr (WIDE) {
+        copied_block<TG>(stages + k * kStageBytes, lane, in);
+        if (add && head) copied_block<TO>(s_added + k * kAddedBytes, lane, there);
+      } else {
+        __syncwarp(mask);  // (what the unit's other lanes have copied)
+        span_block<TG>(stages + k * kStageBytes, row_of(now[k]), a.align, l, in);
+        __syncwarp(mask);
+      }
       if (a.drop.drop_below) add_kept<TG>(sum, in, draws[k % 2], a.drop.drop_below);
       else add_block<TG>(sum, in);
       if (e + kStages < to) issue(e + kStages, k, next[k]);
@@ -484,9 +482,8 @@ int grad(const GradCall& k) {
   HB_CUDA(aside.join());
   a.grads = k.grads;
   a.grad_step = (uint32_t)(k.grad_stride * type_bytes(k.grad_type));
-  const uint64_t ends = (uint64_t)(uintptr_t)k.grads | (uint64_t)(k.grad_stride * type_bytes(k.grad_type)) |
-                        (uint64_t)(k.dim * type_bytes(k.grad_type)) | 16u;
-  a.chunk = (int)(ends & (~ends + 1));
+  const uint64_t starts = (uint64_t)(uintptr_t)k.grads | (uint64_t)a.grad_step | 16u;
+  a.align = (int)(starts & (~starts + 1));
   a.cols = (uint32_t)k.dim;
   a.blocks = p.blocks;
   a.tiles = p.tiles;
@@ -499,8 +496,7 @@ int grad(const GradCall& k) {
   a.num_rows = k.num_rows;
   a.by_run = k.by_run;
   a.num_unique = k.num_unique;
-  const bool wide = a.chunk == 16 && whole_blocks(k.out, k.out_stride, k.out_type, k.dim);
-  if (!wide && a.chunk == 16) a.chunk = 8;
+  const bool wide = a.align == 16 && whole_blocks(k.out, k.out_stride, k.out_type, k.dim);
   const int64_t warps = ceil_div(p.pieces, 32 / p.lanes) * p.tiles, sum_grid = ceil_div(warps, kSumWarps);
   HB_CHECK_ARG(sum_grid < ((int64_t)1 << 31), "%s: more blocks than a launch holds", k.who);
   return with_type(k.grad_type, [&](auto tg) {
