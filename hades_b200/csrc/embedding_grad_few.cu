@@ -14,7 +14,7 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMost = 2048;    // (us, 1,024 bf16 columns into 8,000 rows: 17.0, and one token more in the other form 22.6)
+constexpr int kMost = 2048;    // (us, 1,024 bf16 columns into 8,000 rows: 17.0, in the other form 21.1)
 // Positions of a token that a CTA adds up together, as the longest one that a warp has is what the others wait for (us, 8 / 16 /
 // 32: 512 x 256 fp32 10.3 / 10.3 / 11.6, 2,048 x 1,024 bf16 19.0 / 17.0 / 16.9, 2,048 x 4,096 32.4 / 21.9 / 24.1).
 constexpr int kLong = 16;
@@ -333,14 +333,14 @@ bool whole_rows(const GradCall& k) {
 }  // namespace
 
 // Where the launches that this form spares weigh more than the sums, which the other form's ring of copies feeds better, and
-// than the zeros, which it writes beside its sort (us, this form and the other; 2,048 tokens, bf16: 4,096 columns 22.7 and
-// 24.6, 8,192 29.9 and 27.8, 4,096 with dropout 31.0 and 26.7, 4,001 53.5 and 32.1; 500 of 8,001 23.3 and 23.3; 1,024 of 4,096
-// into 131 MB 35.3 and 37.8, 262 MB 54.1 and 54.5, 1.07 GB 180 and 161).  What is held to fit: token and position a word,
-// bytes of kRows rows of zeros 31 bits.
+// than the zeros, which it writes beside its sort (us, this form and the other; 2,048 tokens, bf16: 4,096 columns 23.2 and
+// 27.3, 6,144 26.6 and 27.0, 8,192 31.5 and 26.0; with dropout 2,048 19.9 and 23.4, 4,096 27.8 and 25.3; ragged 1,001 20.9 and
+// 23.2, 2,001 26.0 and 24.4, 500 tokens of 8,001 25.3 and 21.7; 1,024 of 4,096 into 131 MB 36.2 and 37.1, 262 MB 54.8 and
+// 55.0, 1.07 GB 181 and 161).  What is held to fit: token and position a word, bytes of kRows rows of zeros 31 bits.
 bool grad_few_takes(const GradCall& k, bool dropout) {
   const int64_t row_bytes = k.dim * type_bytes(k.out_type);
   if (k.n <= 0 || k.n > kMost || k.num_rows >= ((int64_t)1 << 32) / (kThreads * entries_each(k)) - 1) return false;
-  if (k.n * k.dim * (whole_rows(k) ? 1 : 2) * (dropout ? 2 : 1) > (8 << 20)) return false;
+  if (k.n * k.dim * (whole_rows(k) ? 1 : 3) * (dropout ? 2 : 1) > (8 << 20)) return false;
   return !k.zeros() || (row_bytes < (1 << 19) && k.num_rows * row_bytes <= (192 << 20));
 }
 
