@@ -4,9 +4,9 @@
 // The tokens are sorted with their positions (runs.cu), and the sorted entries are cut into pieces of equal length, whatever
 // token they hold: a token that is a tenth of all positions costs no warp more than another.  32 lanes take 256 columns of a
 // piece; rows come through a ring of asynchronous copies in shared memory (where rows begin at 16 bytes a lane copies and reads
-// its own eight columns, so that nothing is waited for but the copy), sums stay in registers, and a row leaves as soon as its token ends.  What of a
-// token lies in two pieces or more is left as fp32 partial rows, and whoever leaves the last of them adds them up, in the
-// order of the pieces, so that the bits do not depend on who that is.
+// its own eight columns, so that nothing is waited for but the copy), sums stay in registers, and a row leaves as soon as its
+// token ends.  What of a token lies in two pieces or more is left as fp32 partial rows, and whoever leaves the last of them adds
+// them up, in the order of the pieces, so that the bits do not depend on who that is.
 //
 // What bounds it: for many wide rows HBM, at the 5 TB/s that rows read and written all over the place reach here (65,536 x
 // 1,024 fp16 to fp32 rows: 214 MB in 42 us behind a sort of 27); for fewer the chain sort, look-up of the entries, first rows,
