@@ -12,33 +12,24 @@
 
 namespace hb {
 
-// A stream of this thread on the current device that forks from a stream of the caller's and joins it again.
+// A stream that forks from a stream of the caller's and joins it again.  Each stream of a caller's has one of its own for
+// every thread that calls: of a stream that two of them shared, the second call's work would wait for all that came in front
+// of the first, and two streams that are to run side by side would run one after the other, or wait for one another.
 class Aside {
  public:
   // After everything that `main` holds so far; false: no stream (then nothing is to be launched on it).  Not for captures:
   // the stream would belong to two of them where a thread captures two graphs in turns.
   bool fork(cudaStream_t main) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) return false;
-    Lane& l = lanes().of[dev];
-    if (!l.ready) {
-      if (cudaStreamCreateWithFlags(&l.stream, cudaStreamNonBlocking) != cudaSuccess ||
-          cudaEventCreateWithFlags(&l.forked, cudaEventDisableTiming) != cudaSuccess ||
-          cudaEventCreateWithFlags(&l.done, cudaEventDisableTiming) != cudaSuccess) {
-        cudaGetLastError();
-        return false;
-      }
-      l.ready = true;
-    }
-    if (cudaEventRecord(l.forked, main) != cudaSuccess || cudaStreamWaitEvent(l.stream, l.forked, 0) != cudaSuccess) {
+    Lane* l = lane_of(main);
+    if (!l) return false;
+    if (cudaEventRecord(l->forked, main) != cudaSuccess || cudaStreamWaitEvent(l->stream, l->forked, 0) != cudaSuccess) {
       cudaGetLastError();
       return false;
     }
-    lane_ = &l;
+    lane_ = l;
     main_ = main;
     return true;
   }
-  bool forked() const { return lane_ != nullptr; }
   cudaStream_t stream() const { return lane_->stream; }
   // What comes next on the caller's stream comes behind what was launched on this one.
   cudaError_t join() {
@@ -51,26 +42,59 @@ class Aside {
   ~Aside() { join(); }  // (a call that failed half way)
 
  private:
-  static constexpr int kDevices = 64;
+  static constexpr int kLanes = 64;  // of a thread: streams of callers that come behind those have none
   struct Lane {
+    int device = -1;
+    unsigned long long caller = 0;  // of the caller's stream, which no later stream has (a handle may come again)
     cudaStream_t stream = nullptr;
     cudaEvent_t forked = nullptr, done = nullptr;
-    bool ready = false;
+    bool make() {
+      // (a capture that another thread has begun allows it too)
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      const bool made = cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking) == cudaSuccess &&
+                        cudaEventCreateWithFlags(&forked, cudaEventDisableTiming) == cudaSuccess &&
+                        cudaEventCreateWithFlags(&done, cudaEventDisableTiming) == cudaSuccess;
+      if (!made) {
+        cudaGetLastError();
+        drop();
+      }
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      return made;
+    }
+    void drop() {
+      if (done) cudaEventDestroy(done);
+      if (forked) cudaEventDestroy(forked);
+      if (stream) cudaStreamDestroy(stream);
+      *this = Lane();
+    }
   };
   struct Lanes {
-    Lane of[kDevices];
+    Lane of[kLanes];
+    int made = 0;
     ~Lanes() {  // the end of the thread; fails harmlessly where the runtime is gone
-      for (Lane& l : of)
-        if (l.ready) {
-          cudaEventDestroy(l.forked);
-          cudaEventDestroy(l.done);
-          cudaStreamDestroy(l.stream);
-        }
+      for (int k = 0; k < made; ++k) of[k].drop();
     }
   };
   static Lanes& lanes() {
     static thread_local Lanes t;
     return t;
+  }
+  static Lane* lane_of(cudaStream_t main) {
+    int dev = 0;
+    unsigned long long caller = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaStreamGetId(main, &caller) != cudaSuccess) {
+      cudaGetLastError();
+      return nullptr;
+    }
+    Lanes& t = lanes();
+    for (int k = 0; k < t.made; ++k)
+      if (t.of[k].caller == caller && t.of[k].device == dev) return &t.of[k];
+    if (t.made == kLanes || !t.of[t.made].make()) return nullptr;
+    Lane& l = t.of[t.made++];
+    l.device = dev;
+    l.caller = caller;
+    return &l;
   }
   Lane* lane_ = nullptr;
   cudaStream_t main_ = nullptr;

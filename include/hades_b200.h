@@ -794,8 +794,9 @@ int hb_step_backward(hb_step_t* s, const hb_step_desc_t* d, const int64_t* ids, 
 /* Values are fp32, fp16 or bf16, in any combination of input and output; they    */
 /* are computed in fp32 and rounded once.  Strides count values from one row to   */
 /* the next; the values of a row are contiguous.  The first call on a device      */
-/* allocates its status word, and the first gradient of a thread a stream: make   */
-/* them outside of a stream capture.                                              */
+/* allocates its status word: make it outside of a stream capture.  A gradient    */
+/* outside of captures makes a stream at its first call of a thread on a stream:  */
+/* zeros run there, beside the sort.                                              */
 /* ------------------------------------------------------------------------- */
 #define HB_TYPE_F32 0
 #define HB_TYPE_F16 1
