@@ -1048,7 +1048,9 @@ def cudaEmbeddingGrad(ids, grad, num_embeddings: int, scale: float = 1.0, paddin
                       dtype: torch.dtype | None = None, out=None, accumulate: bool = False):
     """Gradient of the table of ``cudaEmbedding`` from that of its result, [num_embeddings, dim] in dtype (that of grad):
     tokens sorted once, every row of grad read once, sums in fp32 and in the same order every time.  accumulate: added to
-    ``out`` (rows of tokens that do not occur are not touched); else all rows of ``out`` are written."""
+    ``out`` (rows of tokens that do not occur are not touched); else all rows of ``out`` are written.  Should the sort of
+    more than 65,536 tokens give up waiting (HB_ERR_TIMEOUT in ``_lib.device_status()``), the gradient is lost: zeros, or
+    nothing added."""
     return (_lib._NATIVE or _lib.native()).embedding_grad(ids, grad, num_embeddings, scale, padding_idx, dropout, seed, offset,
                                                           rng, dtype, out, accumulate)
 
@@ -1058,7 +1060,8 @@ def cudaEmbeddingGradRows(ids, grad, num_embeddings: int, scale: float = 1.0, pa
                           sync: bool = True):
     """The gradient of ``cudaEmbeddingGrad`` as (distinct tokens ascending, their fp32 rows), cut to their number, which is
     read on the host while the rows are added up.  sync=False: (tokens, rows, number on the device) at full size, for
-    ``SparseAdam.update(tokens, rows, is_unique=True, n_dev=number)``, and in captured graphs."""
+    ``SparseAdam.update(tokens, rows, is_unique=True, n_dev=number)``, and in captured graphs.  A sort that gives up waiting
+    raises; with sync=False the number is 0 and tokens[0] is -1."""
     return (_lib._NATIVE or _lib.native()).embedding_grad_rows(ids, grad, num_embeddings, scale, padding_idx, dropout, seed,
                                                                offset, rng, sync)
 

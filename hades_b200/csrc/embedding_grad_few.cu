@@ -153,7 +153,10 @@ __global__ void __launch_bounds__(kThreads, 1) grad_few_kernel(const FewArgs a) 
   if (t == 0) {
     s_start[runs] = (uint16_t)valid;
     s_ticket = 0;
-    if (a.num_unique && blockIdx.x == 0) *a.num_unique = runs;
+    if (a.num_unique && blockIdx.x == 0) {
+      *a.num_unique = runs;
+      if (runs == 0) a.uniq_ids[0] = a.num_rows;  // (as after the sort of more tokens; -1 there: it gave up)
+    }
   }
   __syncthreads();
   for (int r = t; r < runs; r += kThreads)

@@ -669,6 +669,9 @@ PyObject* embedding_grad_rows(PyObject*, PyObject* const* a, Py_ssize_t n_args) 
                                    rows.data_ptr<float>(), num, ws.data_ptr(), bytes, st));
     if (!sync) return pack({THPVariable_Wrap(uniq), THPVariable_Wrap(rows), THPVariable_Wrap(count)});
     const int64_t u = t_word.wait(static_cast<cudaStream_t>(st));
+    // (none: all of it padding, or nothing to go by)
+    if (u == 0 && uniq.narrow(0, 0, 1).item<int64_t>() < 0)
+      throw std::runtime_error("the sort of the tokens gave up waiting (hb_device_status)");
     return pack({THPVariable_Wrap(uniq.narrow(0, 0, u)), THPVariable_Wrap(rows.narrow(0, 0, u))});
   });
 }

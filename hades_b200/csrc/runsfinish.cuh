@@ -54,6 +54,7 @@ struct RunsFinish {
     *num_runs = *n_valid = run_start[0] = 0;
     run_start[1] = ctx.count;
     uniq[0] = src.sentinel;
+    if (uniq2) uniq2[0] = -1;  // (no id is: entries that all take no part leave the sentinel there)
     if (table) {
       dclass[0] = -1;
       dpos[0] = 0;

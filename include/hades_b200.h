@@ -830,7 +830,9 @@ int hb_dropout(const void* x, int x_type, int64_t x_stride, int64_t n, int64_t d
 /* Gradient of the table of hb_embedding from the gradients of its output: out[v, :] = scale * (sum over the positions i
  * of token v of dropped(grads[i, :])), all num_rows rows, zeros where a token does not occur; accumulate: added to what out
  * holds, rows of other tokens untouched.  Positions of padding_idx or of ids outside of the table (HB_ERR_INVALID in the
- * status word) take no part.  Sums are in fp32 and in the same order every time.  grad_stride below 2^30 values.  workspace:
+ * status word) take no part.  Sums are in fp32 and in the same order every time.  grad_stride below 2^30 values.  The sort
+ * of more than 65,536 positions waits between its CTAs: should that ever run out, HB_ERR_TIMEOUT is in the status word and
+ * the gradient is lost (zeros, or nothing added).  workspace:
  * hb_embedding_grad_workspace_bytes(n, dim), for hb_embedding_grad_rows too (0: sizes that are refused). */
 size_t hb_embedding_grad_workspace_bytes(int64_t n, int64_t dim);
 int hb_embedding_grad(const void* ids, int idx_bytes, int64_t n, int64_t padding_idx, const void* grads, int grad_type,
@@ -840,7 +842,8 @@ int hb_embedding_grad(const void* ids, int idx_bytes, int64_t n, int64_t padding
 
 /* The same as distinct tokens, ascending, and their rows, for a sparse optimiser (hb_sparse_adam / hb_sparse_adagrad with
  * n_dev = num_unique): uniq_ids and rows hold n entries, of which *num_unique (device) are written; the entries of
- * uniq_ids behind them are undefined. */
+ * uniq_ids behind them are undefined, but for the first of a batch (n > 0) without distinct tokens, which is not negative.
+ * Where the sort gave up, *num_unique is 0 and uniq_ids[0] is -1. */
 int hb_embedding_grad_rows(const void* ids, int idx_bytes, int64_t n, int64_t padding_idx, const void* grads,
                            int grad_type, int64_t grad_stride, int64_t dim, double scale,
                            const hb_drop_t* drop /* nullable, host */, int64_t num_rows, int64_t* uniq_ids, float* rows,

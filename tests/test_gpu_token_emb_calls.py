@@ -1,8 +1,14 @@
 """Calls of the token-embedding operators that a program may make beside the usual ones: on several streams, on outputs that
 begin anywhere, by way of other parts of torch."""
+import os
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
+ROOT = Path(__file__).resolve().parent.parent
 pytestmark = pytest.mark.gpu
 
 
@@ -39,3 +45,95 @@ def test_a_gradient_does_not_wait_for_another_stream(E):
             break
     torch.cuda.synchronize()
     assert early and torch.equal(late, want) and all(torch.equal(out, want) for out, _ in outs)
+
+
+# ---- a sort that gives up ---------------------------------------------------------------------------------------------------
+GIVES_UP = r"""
+#include <cstdio>
+#include "runsfinish.cuh"
+
+struct Ctx {
+  static constexpr int kThreads = 64;
+  static constexpr uint32_t count = 100;
+  __device__ uint32_t chunk_begin() const { return 0; }
+  __device__ uint32_t chunk_end() const { return count; }
+};
+struct Source { int64_t sentinel; };
+__global__ void give_up(hb::RunsFinish<false> fin) {
+  Ctx ctx;
+  fin.give_up(ctx, Source{(1 << 20) - 1});
+}
+template <class T> T* words(int n) {
+  T* p = nullptr;
+  cudaMallocManaged(&p, n * sizeof(T));
+  memset(p, 0x55, n * sizeof(T));
+  return p;
+}
+int main() {
+  hb::RunsFinish<false> fin = {};
+  fin.perm = words<uint32_t>(100);
+  fin.head = words<uint8_t>(108);
+  fin.uniq = words<int64_t>(101);
+  fin.uniq2 = words<int64_t>(100);
+  fin.run_start = words<int64_t>(101);
+  fin.num_runs = words<int64_t>(1);
+  fin.num_runs2 = words<int64_t>(1);
+  fin.class_counts = words<int64_t>(4);
+  fin.base8 = words<int32_t>(14);
+  fin.n_valid = words<int64_t>(1);
+  give_up<<<1, 64>>>(fin);
+  if (cudaDeviceSynchronize() != cudaSuccess) return 1;
+  std::printf("%lld %lld %lld %lld", (long long)*fin.num_runs, (long long)*fin.num_runs2, (long long)fin.uniq[0], (long long)fin.uniq2[0]);
+  return 0;
+}
+"""
+
+
+def test_what_a_sort_that_gives_up_leaves(tmp_path):
+    (tmp_path / "up.cu").write_text(GIVES_UP)
+    nvcc = "/usr/local/cuda/bin/nvcc"
+    subprocess.run([nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "--expt-relaxed-constexpr", "--extended-lambda",
+                    "-I", str(ROOT / "include"), "-I", str(ROOT / "hades_b200" / "csrc"), str(tmp_path / "up.cu"),
+                    "-o", str(tmp_path / "up")], check=True, capture_output=True)
+    r = subprocess.run([str(tmp_path / "up")], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and r.stdout == f"0 0 {(1 << 20) - 1} -1", r.stdout + r.stderr
+
+
+# The library's call in the state that such a sort leaves: no tokens, the first of them -1.
+GAVE_UP = r"""
+#include <cstdint>
+#include <cuda_runtime.h>
+extern "C" int hb_embedding_grad_rows(const void*, int, int64_t, int64_t, const void*, int, int64_t, int64_t, double, const void*,
+                                      int64_t, int64_t* uniq, float*, int64_t* num, void*, size_t, cudaStream_t stream) {
+  const int64_t first = FIRST, none = 0;
+  cudaMemcpyAsync(uniq, &first, 8, cudaMemcpyDefault, stream);
+  cudaMemcpyAsync(num, &none, 8, cudaMemcpyDefault, stream);
+  return 0;
+}
+"""
+CALLS = """
+import torch
+from hades_b200 import EmbCacheLib as E
+E.cudaEmbeddingGradRows(torch.zeros(20, dtype=torch.int64, device="cuda"), torch.ones(20, 8, device="cuda"), 4)
+"""
+
+
+def test_a_sort_that_gave_up_is_an_error(tmp_path):
+    for first, raises in ((-1, True), (4, False)):
+        (tmp_path / "up.cpp").write_text(GAVE_UP.replace("FIRST", str(first)))
+        subprocess.run(["g++", "-shared", "-fPIC", "-I", "/usr/local/cuda/include", str(tmp_path / "up.cpp"), "-L",
+                        "/usr/local/cuda/lib64", "-lcudart", "-o", str(tmp_path / f"up{first}.so")], check=True)
+        r = subprocess.run([sys.executable, "-c", CALLS], cwd=ROOT, capture_output=True, text=True, timeout=300,
+                           env={**os.environ, "LD_PRELOAD": str(tmp_path / f"up{first}.so")})
+        assert (r.returncode != 0) == raises and ("gave up waiting" in r.stderr) == raises, r.stderr
+
+
+@pytest.mark.parametrize("n", [100, 2000, 3000, 60_000, 70_000])
+def test_batches_without_tokens(E, n):
+    """Rows of a batch that is all padding: none, and no error; the first token says that the sort did not give up."""
+    ids, g = torch.full((n,), 3, device="cuda"), torch.ones(n, 8, device="cuda")
+    for pad, vocab in ((3, 10), (3, 4)):
+        tokens, rows = E.cudaEmbeddingGradRows(ids, g, vocab, padding_idx=pad)
+        assert tokens.numel() == 0 and rows.shape == (0, 8)
+        tokens, _, number = E.cudaEmbeddingGradRows(ids, g, vocab, padding_idx=pad, sync=False)
+        assert number.item() == 0 and tokens[0].item() >= vocab
