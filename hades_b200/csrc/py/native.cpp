@@ -697,6 +697,9 @@ void refuse_foreign_graphs(const at::Tensor& leaf, const at::Device& dev) {
        "a graph of the same leaf that was built outside of this capture still lives (drop its outputs first)");
 }
 
+// Derivatives in forward mode are not carried: a result without one would count as a derivative of zero.
+void refuse_tangents(const at::Tensor& t) { need(!t._fw_grad(/*level=*/0).defined(), "no derivatives in forward mode"); }
+
 struct TokenNode : public Node {
   SavedVariable ids, rng;
   bool has_ids, captured;
@@ -719,6 +722,7 @@ struct TokenNode : public Node {
     const at::Tensor& g = grads[0];
     if (!g.defined()) return {at::Tensor()};
     need(!(at::GradMode::is_enabled() && g.requires_grad()), "the backward pass is not differentiated again");
+    refuse_tangents(g);
     need(captured || !captures(g.device()), "the forward pass belongs to the capture that its backward pass is in");
     at::AutoGradMode none(false);
     Mask m = mask;
@@ -742,6 +746,7 @@ PyObject* embedding_autograd(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const double scale = number(a[2]);
     const int64_t padding = padding_of(a[3]);
     const at::ScalarType type = type_or(a[8], weight.scalar_type());
+    refuse_tangents(weight);
     const bool track = at::GradMode::is_enabled() && weight.requires_grad();
     if (track && ids.is_cuda()) refuse_foreign_graphs(weight, ids.device());
     at::Tensor out;
@@ -767,6 +772,7 @@ PyObject* dropout_autograd(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const at::Tensor& x = tensor(a[0], "x");
     const Mask mask(a + 2);
     const double scale = number(a[1]);
+    refuse_tangents(x);
     const bool track = at::GradMode::is_enabled() && x.requires_grad();
     if (track && x.is_cuda()) refuse_foreign_graphs(x, x.device());
     at::Tensor out;

@@ -137,3 +137,27 @@ def test_batches_without_tokens(E, n):
         assert tokens.numel() == 0 and rows.shape == (0, 8)
         tokens, _, number = E.cudaEmbeddingGradRows(ids, g, vocab, padding_idx=pad, sync=False)
         assert number.item() == 0 and tokens[0].item() >= vocab
+
+
+# ---- what else torch can do with a call ---------------------------------------------------------------------------------------
+def test_forward_mode_is_refused(E):
+    import torch.autograd.forward_ad as fwd
+
+    from hades_b200 import token_emb
+
+    w, ids = torch.randn(8, 16, device="cuda"), torch.arange(4, device="cuda")
+    with fwd.dual_level():
+        for grad in (False, True):
+            dual = fwd.make_dual(w.clone().requires_grad_(grad), torch.ones_like(w))
+            for call in (lambda: token_emb.embedding(dual, ids), lambda: token_emb.dropout(dual, 0.5)):
+                with pytest.raises(RuntimeError, match="forward mode"):
+                    call()
+        # of a gradient on its way back, too
+        leaf = w.clone().requires_grad_()
+        g = fwd.make_dual(torch.ones(4, 16, device="cuda"), torch.ones(4, 16, device="cuda"))
+        for h in (token_emb.embedding(leaf, ids), token_emb.dropout(leaf, 0.5)[:4]):
+            with pytest.raises(RuntimeError, match="forward mode"):
+                torch.autograd.grad(h, leaf, g)
+        # what has no tangent is as ever, and so is what is taken out of one
+        assert torch.equal(token_emb.embedding(w, ids), w[:4])
+        assert torch.equal(token_emb.embedding(fwd.unpack_dual(fwd.make_dual(w, w)).primal, ids), w[:4])

@@ -1,0 +1,25 @@
+"""What the differentiable token-embedding calls refuse before they look at the device."""
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def token_emb():
+    from hades_b200 import _build, token_emb
+
+    _build.build()
+    return token_emb
+
+
+def test_forward_mode_is_refused(token_emb):
+    import torch.autograd.forward_ad as fwd
+
+    w, ids = torch.randn(8, 16), torch.arange(4)
+    with fwd.dual_level():
+        for grad in (False, True):
+            dual = fwd.make_dual(w.clone().requires_grad_(grad), torch.ones_like(w))
+            for call in (lambda: token_emb.embedding(dual, ids), lambda: token_emb.dropout(dual, 0.5)):
+                with pytest.raises(RuntimeError, match="forward mode"):
+                    call()
+        with pytest.raises(RuntimeError, match="CUDA"):
+            token_emb.embedding(w, ids)
