@@ -7,6 +7,7 @@
 // host a number (how many ids are distinct) while later kernels of the call still run.
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime.h>
@@ -16,6 +17,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <atomic>
 #include <cstring>
@@ -700,6 +702,13 @@ void refuse_foreign_graphs(const at::Tensor& leaf, const at::Device& dev) {
 // Derivatives in forward mode are not carried: a result without one would count as a derivative of zero.
 void refuse_tangents(const at::Tensor& t) { need(!t._fw_grad(/*level=*/0).defined(), "no derivatives in forward mode"); }
 
+// A trace would have the result as a constant: it records what goes through torch's dispatcher.
+void refuse_tracing() {
+  need(!torch::jit::tracer::isTracing() &&
+           !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+       "a trace does not record this call");
+}
+
 struct TokenNode : public Node {
   SavedVariable ids, rng;
   bool has_ids, captured;
@@ -746,6 +755,7 @@ PyObject* embedding_autograd(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const double scale = number(a[2]);
     const int64_t padding = padding_of(a[3]);
     const at::ScalarType type = type_or(a[8], weight.scalar_type());
+    refuse_tracing();
     refuse_tangents(weight);
     const bool track = at::GradMode::is_enabled() && weight.requires_grad();
     if (track && ids.is_cuda()) refuse_foreign_graphs(weight, ids.device());
@@ -772,6 +782,7 @@ PyObject* dropout_autograd(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const at::Tensor& x = tensor(a[0], "x");
     const Mask mask(a + 2);
     const double scale = number(a[1]);
+    refuse_tracing();
     refuse_tangents(x);
     const bool track = at::GradMode::is_enabled() && x.requires_grad();
     if (track && x.is_cuda()) refuse_foreign_graphs(x, x.device());

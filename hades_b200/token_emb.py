@@ -29,7 +29,7 @@ from . import _lib
 def embedding(weight, ids, scale: float = 1.0, padding_idx: int | None = None, dropout: float = 0.0, seed: int = 0,
               offset: int = 0, rng: torch.Tensor | None = None, dtype: torch.dtype | None = None) -> torch.Tensor:
     """``cudaEmbedding``, differentiable (once, in reverse) in weight, all of whose rows the gradient has, zeros where no token
-    points.  Derivatives in forward mode are refused."""
+    points.  Derivatives in forward mode and traces (``torch.jit.trace``, ``make_fx``) are refused."""
     return (_lib._NATIVE or _lib.native()).embedding_autograd(weight, ids, scale, padding_idx, dropout, seed, offset, rng, dtype)
 
 

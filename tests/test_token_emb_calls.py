@@ -23,3 +23,16 @@ def test_forward_mode_is_refused(token_emb):
                     call()
         with pytest.raises(RuntimeError, match="CUDA"):
             token_emb.embedding(w, ids)
+
+
+def test_traces_are_refused(token_emb):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    w, ids = torch.randn(8, 16), torch.arange(4)
+    for call in (lambda a: token_emb.embedding(a, ids), lambda a: token_emb.dropout(a, 0.5)):
+        with torch.no_grad(), pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(call, (w,), check_trace=False)
+        with pytest.raises(RuntimeError, match="trace"):
+            make_fx(call)(w)
+        with pytest.raises(RuntimeError, match="CUDA"):  # (the trace is over)
+            call(w)
