@@ -52,8 +52,8 @@ class DistEmbeddingTensor:
 
     def authoritative_rows(self, ids: torch.Tensor) -> torch.Tensor:
         """Current table rows (no cache), the reference's ``self.tensor[ids]``
-        (dist_emb.py:168-169): from the owners' shards when the table is sharded."""
-        p = self.path
+        (dist_emb.py:168-169), [number of ids, dim]: from the owners' shards when the table is sharded."""
+        p, ids = self.path, ids.reshape(-1)
         if p.shared is not None:
             return p.shared.gather(ids)
         out = torch.empty((ids.numel(), self.embedding_dim), dtype=p.table.dtype, device=ids.device)
@@ -106,7 +106,7 @@ class DistEmb(nn.Module):
         if self.scale == 1.0:
             return self.sparse_emb(idx, None, False)
         if path.shared is None:
-            return E.cudaEmbedding(path.table, idx.to(path.device, non_blocking=True), self.scale)
+            return E.cudaEmbedding(path.table, idx.to(path.device, non_blocking=True).reshape(-1), self.scale)
         return E.cudaDropout(self.sparse_emb(idx, None, False), 0.0, scale=self.scale)
 
 

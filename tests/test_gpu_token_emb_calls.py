@@ -161,3 +161,29 @@ def test_forward_mode_is_refused(E):
         # what has no tangent is as ever, and so is what is taken out of one
         assert torch.equal(token_emb.embedding(w, ids), w[:4])
         assert torch.equal(token_emb.embedding(fwd.unpack_dual(fwd.make_dual(w, w)).primal, ids), w[:4])
+
+
+# ---- DistEmb ------------------------------------------------------------------------------------------------------------------
+def small_path():
+    from hades_b200 import pipeline, synth
+
+    base = synth.scaled(synth.CONFIG1, 0.05, "small")
+    return pipeline.build_path(synth.CacheFetchConfig(base.name, base.config, base.table_rows, base.dim, base.cache_entries,
+                                                      base.batch, base.zipf_s, flush_every=2))
+
+
+def test_dist_emb_has_one_shape(E):
+    """[number of ids, dim] whatever the ids' shape, the scale and the mode."""
+    from hades_b200.dist_emb import DistEmb
+
+    path = small_path()
+    ids = torch.randint(0, path.num_nodes, (7, 30), device="cuda")
+    want = path.table[ids.view(-1)]
+    for given in (ids, ids.t().contiguous().t(), ids.view(-1), ids.view(1, 7, 5, 6), ids.cpu()):
+        for scale in (1.0, 2.0):
+            layer = DistEmb(path, scale=scale, dropout=0.25).eval()
+            assert torch.equal(layer(given), want * scale)
+    assert DistEmb(path, scale=2.0).eval()(ids[0, 0]).shape == DistEmb(path).eval()(ids[0, 0]).shape == (1, path.dim)
+    for scale in (1.0, 2.0):
+        layer = DistEmb(path, scale=scale)
+        assert layer(ids.view(-1)).shape == layer.eval()(ids.view(-1)).shape == (210, path.dim)
