@@ -85,7 +85,8 @@ class DistEmbeddingTensor:
 class DistEmb(nn.Module):
     """``nn.Module`` face of the layer (dist_emb.py:11-51).  scale, dropout (not in the reference; rows of fp32, fp16 or
     bf16): what it returns is scale times the rows, in training with a share ``dropout`` of the values dropped
-    (``token_emb.dropout``, seeded by ``seed``); gradients reach the rows through both."""
+    (``token_emb.dropout``, seeded by ``seed``); gradients reach the rows through both.  With dropout a forward pass that is
+    run again within a backward pass (activation checkpointing) is refused: its mask would be another one."""
 
     def __init__(self, path: EmbeddingPath, name: str = "emb_layer", scale: float = 1.0, dropout: float = 0.0,
                  seed: int | None = None):

@@ -53,7 +53,11 @@ class DropoutSeeds:
             self.state = torch.tensor([self.seed, 0], dtype=torch.int64, device=on_device)
 
     def next(self) -> dict:
-        """The next mask, as the arguments of ``cudaDropout`` and its like."""
+        """The next mask, as the arguments of ``cudaDropout`` and its like.  Not within a backward pass: a forward pass that
+        is run again there (activation checkpointing) needs the mask that it had."""
+        E._check(torch._C._current_graph_task_id() == -1,
+                 "a forward pass that runs again within a backward pass (activation checkpointing) would draw another mask: "
+                 "call token_emb.embedding or token_emb.dropout with a seed and an offset of your own there")
         if self.state is None:
             self.offset += 1
             return {"seed": self.seed, "offset": self.offset}
@@ -72,8 +76,8 @@ class DropoutSeeds:
 
 class TokenEmbedding(nn.Module):
     """A table of [num_embeddings, embedding_dim] weights on the GPU, looked up by token.  Values are multiplied by
-    ``scale``; in training a share ``dropout`` of them is dropped.  Every forward pass draws another mask, one that is
-    computed again for a backward pass (activation checkpointing) too: call ``embedding`` with numbers of your own there."""
+    ``scale``; in training a share ``dropout`` of them is dropped.  Every forward pass draws another mask; one that is run
+    again within a backward pass (activation checkpointing) is refused: call ``embedding`` with numbers of your own there."""
 
     def __init__(self, num_embeddings: int, embedding_dim: int, scale: float = 1.0, padding_idx: int | None = None,
                  dropout: float = 0.0, dtype=torch.float32, device="cuda", init_sigma: float = 0.02, seed: int | None = None,

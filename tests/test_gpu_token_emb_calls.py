@@ -187,3 +187,29 @@ def test_dist_emb_has_one_shape(E):
     for scale in (1.0, 2.0):
         layer = DistEmb(path, scale=scale)
         assert layer(ids.view(-1)).shape == layer.eval()(ids.view(-1)).shape == (210, path.dim)
+
+
+def test_checkpointed_layers(E):
+    from torch.utils.checkpoint import checkpoint
+
+    from hades_b200 import token_emb
+
+    layer, ids = token_emb.TokenEmbedding(40, 64, dropout=0.5, seed=1), torch.randint(0, 40, (50,), device="cuda")
+    for reentrant in (False, True):
+        x = torch.ones((), device="cuda", requires_grad=True)
+        h = checkpoint(lambda x: (layer(ids) * x).sin(), x, use_reentrant=reentrant)
+        with pytest.raises(RuntimeError, match="another mask"):
+            h.sum().backward()
+        layer.weight.grad = None
+        # with numbers of one's own, and without dropout, as without checkpoints
+        for p in (0.5, 0.0):
+            def passes(x, p=p):
+                return (token_emb.embedding(layer.weight, ids, dropout=p, seed=1, offset=9) * x).sin()
+
+            want = torch.autograd.grad(passes(x).sum(), layer.weight)[0]
+            checkpoint(passes, x, use_reentrant=reentrant).sum().backward()
+            assert torch.equal(layer.weight.grad, want)
+            layer.weight.grad = None
+    layer.eval()
+    checkpoint(lambda x: (layer(ids) * x).sin(), x, use_reentrant=False).sum().backward()
+    assert layer.weight.grad is not None

@@ -36,3 +36,23 @@ def test_traces_are_refused(token_emb):
             make_fx(call)(w)
         with pytest.raises(RuntimeError, match="CUDA"):  # (the trace is over)
             call(w)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_masks_of_passes_that_run_again_are_refused(token_emb, reentrant):
+    from torch.utils.checkpoint import checkpoint
+
+    seeds, drawn = token_emb.DropoutSeeds(3), []
+
+    def layer(x):
+        drawn.append(seeds.next())
+        return (x * drawn[-1]["offset"]).sin()
+
+    x = torch.ones(4, requires_grad=True)
+    y = checkpoint(layer, x, use_reentrant=reentrant)
+    with pytest.raises(RuntimeError, match="another mask"):
+        y.sum().backward()
+    assert len(drawn) == 1 and seeds.next()["offset"] == 2
+    mask = seeds.next()  # numbers of one's own
+    checkpoint(lambda x: (x * mask["offset"]).sin(), x, use_reentrant=reentrant).sum().backward()
+    assert x.grad is not None
