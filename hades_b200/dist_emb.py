@@ -21,7 +21,6 @@ accumulate, exchange, update, periodic flush) and returns its counters.
 from __future__ import annotations
 
 import torch
-import torch.nn as nn
 
 from . import EmbCacheLib as E
 from . import token_emb
@@ -82,7 +81,7 @@ class DistEmbeddingTensor:
         self.trace = []
 
 
-class DistEmb(nn.Module):
+class DistEmb(token_emb.MaskedModule):
     """``nn.Module`` face of the layer (dist_emb.py:11-51).  scale, dropout (not in the reference; rows of fp32, fp16 or
     bf16): what it returns is scale times the rows, in training with a share ``dropout`` of the values dropped
     (``token_emb.dropout``, seeded by ``seed``); gradients reach the rows through both.  With dropout a forward pass that is

@@ -73,8 +73,45 @@ class DropoutSeeds:
         if self.state is not None:
             self.state.copy_(torch.tensor([self.seed, self.offset]))
 
+    def to(self, device) -> None:
+        """Moves what is kept on a GPU (a captured graph goes on with the tensor that it was captured with)."""
+        if self.state is not None and torch.device(device).type != "meta":
+            self.state = self.state.to(device)
 
-class TokenEmbedding(nn.Module):
+
+class MaskedModule(nn.Module):
+    """A module that drops a share ``dropout`` of its values by ``seeds``: seed and number of masks are saved with it and move
+    with it, so that a run that continues draws the next mask.  (Ranks that all load one state draw the same masks from
+    there on.)  A state without them leaves them as they are."""
+
+    def get_extra_state(self) -> torch.Tensor:
+        s = self.seeds
+        if s is None or s.state is None:
+            return torch.tensor([s.seed, s.offset] if s else [])
+        return s.state.clone()
+
+    def set_extra_state(self, state: torch.Tensor) -> None:
+        if self.dropout:
+            seed, offset = state.tolist()
+            self.seeds.load_state_dict({"seed": seed, "offset": offset})
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        if not self.dropout:
+            del destination[prefix + "_extra_state"]
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, *args):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, *args)
+        missing_keys[:] = [key for key in missing_keys if key != prefix + "_extra_state"]
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        if self.seeds is not None and self.seeds.state is not None:
+            self.seeds.to(fn(self.seeds.state).device)
+        return self
+
+
+class TokenEmbedding(MaskedModule):
     """A table of [num_embeddings, embedding_dim] weights on the GPU, looked up by token.  Values are multiplied by
     ``scale``; in training a share ``dropout`` of them is dropped.  Every forward pass draws another mask; one that is run
     again within a backward pass (activation checkpointing) is refused: call ``embedding`` with numbers of your own there."""

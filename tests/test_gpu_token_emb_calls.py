@@ -213,3 +213,17 @@ def test_checkpointed_layers(E):
     layer.eval()
     checkpoint(lambda x: (layer(ids) * x).sin(), x, use_reentrant=False).sum().backward()
     assert layer.weight.grad is not None
+
+
+def test_a_layer_that_was_saved_draws_the_next_mask(E):
+    from hades_b200.token_emb import TokenEmbedding
+
+    ids = torch.randint(0, 40, (50,), device="cuda")
+    for on_device in (False, True):
+        make = lambda seed: TokenEmbedding(40, 64, dropout=0.5, seed=seed, seed_on_device=on_device)  # noqa: E731
+        layer, other = make(3), make(4)
+        layer(ids)
+        other.load_state_dict(layer.state_dict())
+        assert torch.equal(layer(ids), other(ids))
+        moved = layer.cpu().cuda()
+        assert torch.equal(moved(ids), other(ids)) and (not on_device or moved.seeds.state.is_cuda)

@@ -56,3 +56,66 @@ def test_masks_of_passes_that_run_again_are_refused(token_emb, reentrant):
     mask = seeds.next()  # numbers of one's own
     checkpoint(lambda x: (x * mask["offset"]).sin(), x, use_reentrant=reentrant).sum().backward()
     assert x.grad is not None
+
+
+def _layer(token_emb, **kw):
+    return token_emb.TokenEmbedding(4, 8, device="cpu", **kw)
+
+
+def test_masks_are_saved_with_the_layer(token_emb, tmp_path):
+    """A run that continues from a module's state draws the next mask, not the first."""
+    for make in (lambda seed: _layer(token_emb, dropout=0.5, seed=seed), lambda seed: _dist_emb(0.5, seed)):
+        layer = make(7)
+        model = torch.nn.Sequential(torch.nn.Linear(2, 2), layer)
+        drawn = [layer.seeds.next() for _ in range(3)]
+        torch.save(model.state_dict(), tmp_path / "state")
+        assert drawn[-1] == {"seed": 7, "offset": 3}
+        state = torch.load(tmp_path / "state")  # (tensors only)
+        for seed in (7, None):
+            other = torch.nn.Sequential(torch.nn.Linear(2, 2), make(seed))
+            other.load_state_dict(state)
+            assert other[1].seeds.next() == {"seed": 7, "offset": 4}
+        largest = make((1 << 63) - 1)
+        copy = make(0)
+        copy.load_state_dict(largest.state_dict())
+        assert copy.seeds.next() == {"seed": (1 << 63) - 1, "offset": 1}
+        # as saved before the numbers were: nothing is missing, and they stay
+        for key in [k for k in state if "extra" in k]:
+            del state[key]
+        other.load_state_dict(state)
+        assert other[1].seeds.next() == {"seed": 7, "offset": 5}
+
+
+def _dist_emb(dropout, seed=None):
+    from types import SimpleNamespace
+
+    from hades_b200.dist_emb import DistEmb
+
+    return DistEmb(SimpleNamespace(dim=8, num_nodes=4), dropout=dropout, seed=seed)
+
+
+def test_layers_without_dropout_save_what_they_did(token_emb):
+    plain, dropping = _layer(token_emb), _layer(token_emb, dropout=0.5, seed=1)
+    assert list(plain.state_dict()) == ["weight"] and not _dist_emb(0.0).state_dict()
+    dropping.load_state_dict(plain.state_dict())
+    plain.load_state_dict(dropping.state_dict())
+    assert torch.equal(plain.weight, dropping.weight) and dropping.seeds.next() == {"seed": 1, "offset": 1}
+    _dist_emb(0.0).load_state_dict(_dist_emb(0.5).state_dict())
+    with pytest.raises(RuntimeError, match="Missing key"):
+        plain.load_state_dict({})
+    with pytest.raises(RuntimeError, match="Unexpected key"):
+        plain.load_state_dict({**plain.state_dict(), "other": torch.zeros(1)})
+
+
+def test_numbers_on_a_device_move_with_the_layer(token_emb):
+    layer = _layer(token_emb, dropout=0.5, seed=5, seed_on_device=True)
+    layer.seeds.next()
+    kept = layer.seeds.state
+    layer.half().to("cpu").double()
+    assert layer.seeds.state is kept and kept.tolist() == [5, 1] and kept.dtype == torch.int64
+    other = _layer(token_emb, dropout=0.5, seed=6, seed_on_device=True)
+    at = other.seeds.state.data_ptr()
+    other.load_state_dict(layer.state_dict())
+    assert other.seeds.next()["rng"].tolist() == [5, 2] and other.seeds.state.data_ptr() == at
+    layer.to("meta")  # has no numbers to keep
+    assert layer.seeds.state.tolist() == [5, 1]
