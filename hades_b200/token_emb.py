@@ -112,16 +112,17 @@ class MaskedModule(nn.Module):
 
 
 class TokenEmbedding(MaskedModule):
-    """A table of [num_embeddings, embedding_dim] weights on the GPU, looked up by token.  Values are multiplied by
-    ``scale``; in training a share ``dropout`` of them is dropped.  Every forward pass draws another mask; one that is run
-    again within a backward pass (activation checkpointing) is refused: call ``embedding`` with numbers of your own there."""
+    """A table of [num_embeddings, embedding_dim] weights on the GPU, looked up by token, results in ``out_dtype`` (None: the
+    weights').  Values are multiplied by ``scale``; in training a share ``dropout`` of them is dropped.  Every forward pass
+    draws another mask; one that is run again within a backward pass (activation checkpointing) is refused: call
+    ``embedding`` with numbers of your own there."""
 
     def __init__(self, num_embeddings: int, embedding_dim: int, scale: float = 1.0, padding_idx: int | None = None,
                  dropout: float = 0.0, dtype=torch.float32, device="cuda", init_sigma: float = 0.02, seed: int | None = None,
-                 seed_on_device: bool = False):
+                 seed_on_device: bool = False, out_dtype: torch.dtype | None = None):
         super().__init__()
         E._check(0.0 <= dropout <= 1.0, "0 <= dropout <= 1")
-        self.scale, self.padding_idx, self.dropout = float(scale), padding_idx, float(dropout)
+        self.scale, self.padding_idx, self.dropout, self.out_dtype = float(scale), padding_idx, float(dropout), out_dtype
         weight = torch.empty((num_embeddings, embedding_dim), dtype=dtype, device=device).normal_(0.0, init_sigma)
         if padding_idx is not None and 0 <= padding_idx < num_embeddings:
             weight[padding_idx].zero_()
@@ -130,4 +131,4 @@ class TokenEmbedding(MaskedModule):
 
     def forward(self, ids: torch.Tensor) -> torch.Tensor:
         drop = {"dropout": self.dropout, **self.seeds.next()} if self.training and self.dropout else {}
-        return embedding(self.weight, ids, self.scale, self.padding_idx, **drop)
+        return embedding(self.weight, ids, self.scale, self.padding_idx, dtype=self.out_dtype, **drop)

@@ -227,3 +227,20 @@ def test_a_layer_that_was_saved_draws_the_next_mask(E):
         assert torch.equal(layer(ids), other(ids))
         moved = layer.cpu().cuda()
         assert torch.equal(moved(ids), other(ids)) and (not on_device or moved.seeds.state.is_cuda)
+
+
+@pytest.mark.parametrize("weights,results", [(torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32),
+                                             (torch.float16, None)])
+def test_the_type_of_a_layers_results(E, weights, results):
+    from hades_b200.token_emb import TokenEmbedding
+
+    layer = TokenEmbedding(40, 64, scale=2.0, padding_idx=0, dropout=0.5, dtype=weights, seed=3, out_dtype=results)
+    ids = torch.randint(0, 40, (6, 50), device="cuda")
+    h = layer(ids)
+    assert h.dtype == (results or weights)
+    assert torch.equal(h, E.cudaEmbedding(layer.weight.detach(), ids, 2.0, 0, 0.5, seed=3, offset=1, dtype=results))
+    g = torch.randn_like(h)
+    h.backward(g)
+    want = E.cudaEmbeddingGrad(ids, g, 40, 2.0, 0, 0.5, seed=3, offset=1, dtype=weights)
+    assert layer.weight.grad.dtype == weights and torch.equal(layer.weight.grad, want)
+    assert layer.eval()(ids).dtype == (results or weights)
