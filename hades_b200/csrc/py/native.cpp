@@ -504,6 +504,7 @@ struct Mask {
 // [rows, dim] of a tensor whose last dimension is dim: the distance of its rows, or -1 where they are not evenly spaced.
 int64_t row_stride(const at::Tensor& t) {
   const int64_t k = t.dim();
+  if (k > 0 && t.numel() == 0) return t.size(k - 1);  // no rows
   if (k == 0 || (t.size(k - 1) > 1 && t.stride(k - 1) != 1)) return -1;
   int64_t stride = 0, rows = 1;  // rows of the inner dimensions so far
   for (int64_t d = k - 2; d >= 0; --d) {

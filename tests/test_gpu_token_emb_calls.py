@@ -244,3 +244,14 @@ def test_the_type_of_a_layers_results(E, weights, results):
     want = E.cudaEmbeddingGrad(ids, g, 40, 2.0, 0, 0.5, seed=3, offset=1, dtype=weights)
     assert layer.weight.grad.dtype == weights and torch.equal(layer.weight.grad, want)
     assert layer.eval()(ids).dtype == (results or weights)
+
+
+def test_empty_results_into_a_given_tensor(E):
+    w = torch.randn(8, 16, device="cuda")
+    for shape in ((0,), (2, 0), (0, 3), (2, 0, 3), (0, 0)):
+        ids, out = torch.zeros(shape, dtype=torch.int64, device="cuda"), torch.empty((*shape, 16), device="cuda")
+        assert E.cudaEmbedding(w, ids, out=out).data_ptr() == out.data_ptr()
+        assert E.cudaDropout(out, 0.5, out=torch.empty_like(out)).shape == out.shape
+        grad = E.cudaEmbeddingGrad(ids, out, 8, out=torch.ones_like(w), accumulate=True)
+        assert bool((grad == 1).all())
+        assert E.cudaEmbeddingGrad(ids, out, 0, out=w[:0]).shape == (0, 16)
