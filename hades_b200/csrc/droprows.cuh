@@ -34,6 +34,7 @@ static inline int dropout_of(const char* who, double scale, const hb_drop_t* dro
   HB_CHECK_ARG(!drop || (drop->p >= 0.0 && drop->p <= 1.0), "%s: the dropout probability must be in [0, 1]", who);
   const double t = drop ? std::floor(drop->p * 65536.0 + 0.5) : 0.0;
   const double f = t < 65536.0 ? scale * 65536.0 / (65536.0 - t) : 0.0;
+  HB_CHECK_ARG(!drop || ((uintptr_t)drop->rng & 7) == 0, "%s: seed and offset are not aligned", who);
   HB_CHECK_ARG(std::isfinite(scale) && std::isfinite((float)f), "%s: the scale must be finite", who);
   out->drop_below = (uint32_t)t;
   out->factor = (float)f;
@@ -45,6 +46,9 @@ static inline int dropout_of(const char* who, double scale, const hb_drop_t* dro
 
 static inline int type_bytes(int type) { return type == HB_TYPE_F32 ? 4 : 2; }
 static inline bool type_known(int type) { return type == HB_TYPE_F32 || type == HB_TYPE_F16 || type == HB_TYPE_BF16; }
+
+// Whether what lies at p begins where its values of so many bytes can.
+static inline bool aligned(const void* p, int64_t bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
 
 // Whether matrices of rows of dim values share memory (as ranges of addresses).
 static inline bool overlap(const void* a, int64_t a_stride, int a_type, int64_t a_rows, const void* b, int64_t b_stride,

@@ -245,6 +245,8 @@ int hb_embedding(const void* weight, int weight_type, int64_t weight_stride, int
   HB_CHECK_ARG(type_known(weight_type) && type_known(out_type), "hb_embedding: unknown value type");
   HB_CHECK_ARG(idx_bytes == 4 || idx_bytes == 8, "hb_embedding: idx_bytes must be 4 or 8");
   HB_CHECK_ARG(n == 0 || (ids && out && (weight || num_rows == 0)), "hb_embedding: null argument");
+  HB_CHECK_ARG(aligned(ids, idx_bytes) && aligned(weight, type_bytes(weight_type)) && aligned(out, type_bytes(out_type)),
+               "hb_embedding: ids, table or output not aligned to their values");
   HB_CHECK_ARG(weight_stride >= 0, "hb_embedding: bad table stride");
   HB_CHECK_ARG(out_stride >= dim || n <= 1, "hb_embedding: output rows overlap");
   LookupArgs a = {};
@@ -269,6 +271,8 @@ int hb_dropout(const void* x, int x_type, int64_t x_stride, int64_t n, int64_t d
   HB_CHECK_ARG(n >= 0 && n <= ((int64_t)1 << 32) && dim > 0 && dim < ((int64_t)1 << 24), "hb_dropout: bad sizes");
   HB_CHECK_ARG(type_known(x_type) && type_known(y_type), "hb_dropout: unknown value type");
   HB_CHECK_ARG(n == 0 || (x && y), "hb_dropout: null argument");
+  HB_CHECK_ARG(aligned(x, type_bytes(x_type)) && aligned(y, type_bytes(y_type)),
+               "hb_dropout: input or output not aligned to its values");
   HB_CHECK_ARG(x_stride >= 0 && (y_stride >= dim || n <= 1), "hb_dropout: output rows overlap");
   LookupArgs a = {};
   const int rc = dropout_of("hb_dropout", scale, drop, &a.drop);

@@ -418,6 +418,9 @@ int check_call(const GradCall& k) {
   HB_CHECK_ARG(type_known(k.grad_type) && type_known(k.out_type), "%s: unknown value type", k.who);
   HB_CHECK_ARG(k.idx_bytes == 4 || k.idx_bytes == 8, "%s: idx_bytes must be 4 or 8", k.who);
   HB_CHECK_ARG(k.n == 0 || (k.ids && k.grads), "%s: null argument", k.who);
+  HB_CHECK_ARG(aligned(k.ids, k.idx_bytes) && aligned(k.grads, type_bytes(k.grad_type)) && aligned(k.out, type_bytes(k.out_type)) &&
+                   aligned(k.uniq_ids, 8) && aligned(k.num_unique, 8) && aligned(k.ws, 16),
+               "%s: ids, gradients or outputs not aligned to their values, or the workspace to 16 bytes", k.who);
   HB_CHECK_ARG(k.grad_stride >= 0 && k.grad_stride < ((int64_t)1 << 30), "%s: bad gradient stride", k.who);
   HB_CHECK_ARG(!k.out || !overlap(k.grads, k.grad_stride, k.grad_type, k.n, k.out, k.out_stride, k.out_type,
                                   k.by_run ? k.n : k.num_rows, k.dim),

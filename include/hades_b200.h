@@ -793,7 +793,8 @@ int hb_step_backward(hb_step_t* s, const hb_step_desc_t* d, const int64_t* ids, 
 /* rows, python/EmbCache/dist_emb.py:199-212).                                    */
 /* Values are fp32, fp16 or bf16, in any combination of input and output; they    */
 /* are computed in fp32 and rounded once.  Strides count values from one row to   */
-/* the next; the values of a row are contiguous.  The first call on a device      */
+/* the next; the values of a row are contiguous.  Pointers are aligned to what    */
+/* they point to, a workspace to 16 bytes.  The first call on a device            */
 /* allocates its status word: make it outside of a stream capture.  A gradient    */
 /* outside of captures makes a stream at its first call of a thread on a stream:  */
 /* zeros run there, beside the sort.                                              */

@@ -11,6 +11,32 @@ def token_emb():
     return token_emb
 
 
+A = 1 << 20  # made-up addresses: the calls return before anything that they point to is looked at
+
+
+def test_pointers_between_values_are_refused(token_emb):
+    import ctypes as C
+
+    from hades_b200 import _lib
+
+    lib = _lib.load()
+    refused = lambda rc: rc == 1 and b"aligned" in lib.hb_last_error()  # noqa: E731
+    drop = C.byref(_lib.DropDesc(0.5, 0, 0, A + 4))
+    for t, between in ((0, 2), (0, 1), (1, 1), (2, 1)):
+        for k in range(3):
+            w, ids, out = (A * (i + 1) + (between if i == k else 0) for i in range(3))
+            assert refused(lib.hb_embedding(w, t, 16, 100, 16, ids, 4, 10, -1, 1.0, None, out, t, 16, None))
+            assert k == 1 or refused(lib.hb_dropout(w, t, 16, 10, 16, 1.0, None, out, t, 16, None))
+            assert refused(lib.hb_embedding_grad(ids, 8, 10, -1, w, t, 16, 16, 1.0, None, 100, out, t, 16, 0, 4 * A, 1 << 30, None))
+    assert refused(lib.hb_embedding(A, 0, 16, 100, 16, 2 * A, 8, 10, -1, 1.0, drop, 3 * A, 0, 16, None))
+    assert refused(lib.hb_dropout(A, 0, 16, 10, 16, 1.0, drop, 2 * A, 0, 16, None))
+    assert refused(lib.hb_embedding_grad(A, 8, 10, -1, 2 * A, 0, 16, 16, 1.0, drop, 100, 3 * A, 0, 16, 0, 4 * A, 1 << 30, None))
+    assert refused(lib.hb_embedding_grad(A, 8, 10, -1, 2 * A, 0, 16, 16, 1.0, None, 100, 3 * A, 0, 16, 0, 4 * A + 8, 1 << 30, None))
+    for k, between in enumerate((4, 2, 4, 8)):
+        uniq, rows, num, ws = ((5 + i) * A + (between if i == k else 0) for i in range(4))
+        assert refused(lib.hb_embedding_grad_rows(A, 8, 10, -1, 2 * A, 0, 16, 16, 1.0, None, 100, uniq, rows, num, ws, 1 << 30, None))
+
+
 def test_forward_mode_is_refused(token_emb):
     import torch.autograd.forward_ad as fwd
 
