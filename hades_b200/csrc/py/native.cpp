@@ -476,6 +476,11 @@ double number(PyObject* o) {
   if (v == -1.0 && PyErr_Occurred()) throw Status();
   return v;
 }
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw Status();
+  return v != 0;
+}
 uint64_t word64(PyObject* o) {  // OverflowError outside of [0, 2^64)
   const unsigned long long v = PyLong_AsUnsignedLongLong(o);
   if (v == (unsigned long long)-1 && PyErr_Occurred()) throw Status();
@@ -639,7 +644,7 @@ PyObject* embedding_grad(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return guarded([&]() -> PyObject* {
     arity(n_args, 12, "embedding_grad");
     const GradInputs in(tensor(a[0], "ids"), tensor(a[1], "grad"), integer(a[2]));
-    const bool accumulate = PyObject_IsTrue(a[11]);
+    const bool accumulate = truth(a[11]);
     need(!accumulate || !none(a[10]), "accumulate adds to a given out");
     const at::Tensor out = optional_tensor(a[10], "out");
     return THPVariable_Wrap(run_embedding_grad(in, number(a[3]), padding_of(a[4]), Mask(a + 5),
@@ -653,7 +658,7 @@ PyObject* embedding_grad_rows(PyObject*, PyObject* const* a, Py_ssize_t n_args) 
   return guarded([&]() -> PyObject* {
     arity(n_args, 10, "embedding_grad_rows");
     const GradInputs in(tensor(a[0], "ids"), tensor(a[1], "grad"), integer(a[2]));
-    const bool sync = PyObject_IsTrue(a[9]);
+    const bool sync = truth(a[9]);
     c10::cuda::CUDAGuard guard(in.dev);
     void* st = stream_of(in.dev);
     cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;

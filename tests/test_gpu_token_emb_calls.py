@@ -255,3 +255,13 @@ def test_empty_results_into_a_given_tensor(E):
         grad = E.cudaEmbeddingGrad(ids, out, 8, out=torch.ones_like(w), accumulate=True)
         assert bool((grad == 1).all())
         assert E.cudaEmbeddingGrad(ids, out, 0, out=w[:0]).shape == (0, 16)
+
+
+def test_flags_that_are_neither_true_nor_false(E):
+    ids, g = torch.arange(4, device="cuda"), torch.ones(4, 16, device="cuda")
+    out = torch.zeros(8, 16, device="cuda")
+    for call in (lambda: E.cudaEmbeddingGrad(ids, g, 8, out=out, accumulate=torch.ones(2)),
+                 lambda: E.cudaEmbeddingGradRows(ids, g, 8, sync=torch.ones(2))):
+        with pytest.raises(RuntimeError, match="ambiguous"):
+            call()
+    assert not out.any()
