@@ -265,3 +265,47 @@ def test_flags_that_are_neither_true_nor_false(E):
         with pytest.raises(RuntimeError, match="ambiguous"):
             call()
     assert not out.any()
+
+
+# ---- zeros of the rows that no token points to ----------------------------------------------------------------------------------
+def check_every_row(E, out, ids, g, **call):
+    """Into an output that held NaN, against sums in 64 bits: m terms in any order are within (m - 1) 2^-24 of the sum of their
+    magnitudes, the result is rounded once more (eps / 2), and where there is no term it is +0."""
+    assert bool(out.isnan().all())
+    E.cudaEmbeddingGrad(ids, g, out.shape[0], out=out, **call)
+    want = torch.zeros(out.shape, dtype=torch.float64, device="cuda").index_add_(0, ids, g.double())
+    size = torch.zeros_like(want).index_add_(0, ids, g.double().abs())
+    terms = torch.bincount(ids, minlength=out.shape[0]).double()[:, None]
+    bound = (terms - 1).clamp(min=0) * 2.0 ** -24 * (1 + 2.0 ** -20) * size
+    bound = bound + torch.finfo(out.dtype).eps / 2 * (want.abs() + bound) + {2: 2.0 ** -25, 4: 2.0 ** -150}[out.element_size()]
+    assert bool(((out.double() - want).abs() <= bound).all())
+    absent = out[terms[:, 0] == 0]
+    assert not absent.any() and not torch.signbit(absent).any()
+
+
+@pytest.mark.parametrize("n,vocab,dim", [
+    (500, 3_000, 64), (500, 2_000, 20_011),   # few tokens; few of many bytes
+    (5_000, 9_000, 100), (30_000, 60_000, 513),  # zeros beside the sort of one cluster, 123 MB of them
+    (70_000, 9_000, 100), (70_000, 60_000, 513)])  # beside the sort of the whole GPU, and in front of it
+@pytest.mark.parametrize("t", [torch.float32, torch.float16])
+def test_every_row_is_written(E, n, vocab, dim, t):
+    torch.manual_seed(n + dim)
+    ids = torch.randint(0, vocab // 2, (n,), device="cuda") * 2  # every other row, the last one among the others
+    g = torch.randn(n, dim, device="cuda").to(t)
+    check_every_row(E, torch.full((vocab, dim), float("nan"), dtype=t, device="cuda"), ids, g)
+    wide = torch.full((vocab, dim + 3), float("nan"), dtype=t, device="cuda")  # rows at a distance
+    check_every_row(E, wide[:, 1:dim + 1], ids, g)
+    assert bool(wide[:, 0].isnan().all()) and bool(wide[:, dim + 1:].isnan().all())
+
+
+@pytest.mark.parametrize("n", [100, 3_000, 70_000])
+@pytest.mark.parametrize("vocab,dim", [(50, 1001), (7, 3), (300, 1)])
+def test_zeros_of_a_stretch_that_begins_anywhere(E, n, vocab, dim):
+    """Two-byte values from 1 to 8 values behind a boundary of 16 bytes on; the first and the last rows have no tokens."""
+    torch.manual_seed(dim)
+    ids = torch.randint(2, vocab - 2, (n,), device="cuda")
+    g = torch.randn(n, dim, device="cuda").half()
+    for first in range(9):
+        base = torch.full((vocab * dim + 24,), float("nan"), dtype=torch.float16, device="cuda")
+        check_every_row(E, base[first:first + vocab * dim].view(vocab, dim), ids, g)
+        assert bool(base[:first].isnan().all()) and bool(base[first + vocab * dim:].isnan().all())
