@@ -6,8 +6,9 @@
 // (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011): counter (column / 8, row, offset's
 // low and high word), key the seed.  A call's 128 bits are the draws of eight neighbouring columns, so that a place needs
 // no state and no mask in memory, and forward and backward passes agree whatever kernel or layout they use.  Ten rounds and
-// the eight selections are 78 of the 138 instructions that a block of bf16 values takes (65,536 x 4,096: 159 us without, 180
-// with dropout, at 62 % of the ALU's and of the wide multipliers' cycles); 32 bits a value would need twice the rounds.
+// the eight selections are 78 of the 138 instructions that a block of bf16 values takes (65,536 x 4,096: 162 us without, 182
+// with dropout, at 62 % of the ALU's and of the wide multipliers' cycles; 195 to 200 where L2 is full of lines that have yet
+// to be written); 32 bits a value would need twice the rounds.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -6,10 +6,12 @@
 // the largest pieces that the rows' starts and ends allow; single words leave through shared memory, halves in pairs that
 // neighbouring lanes exchange.
 //
-// What bounds it: few rows the launch (2 us); many the way between the SMs and L2, where a token's row comes by as often as
-// it occurs (16,384 x 4,096 bf16: 268 MB in 35 us; 32,768 x 2,048 fp32 to bf16 with dropout 403 MB in 53), or HBM (dropout of
-// 65,536 x 4,096 bf16: 1.07 GB in 180 us, 159 without dropout); ragged rows the issue of their pieces (10,007 x 1,001 fp16 to
-// fp32: 15 us at 75 % of all slots).
+// What bounds it: few rows the launch (2 us).  Many without dropout HBM (65,536 distinct tokens x 4,096 bf16: 1.07 GB in 166
+// us), or, where rows come again and again, no unit alone (16,384 x 4,096 bf16 of 3,800 tokens 37 us, 32,768 x 2,048 fp32 to
+// bf16 of 6,900 tokens 43: L1, L2 and HBM at 40 to 55 % of their peaks, 45 to 60 % of issue slots).  With dropout the
+// generator's instructions (the same two 55 us and 55: 70 % of issue slots, 60 % of the ALU's and of the wide multipliers'
+// cycles, L2 at 30 %; dropout alone of 65,536 x 4,096 bf16 182).  Ragged rows the issue of their pieces (10,007 x 1,001 fp16
+// to fp32: 16 us at 75 % of all slots, 79 % of L1).
 #include "droprows.cuh"
 
 namespace hb {
@@ -19,7 +21,10 @@ namespace {
 
 constexpr int kThreads = 128;  // (us, dropout of 65,536 x 4,096 bf16: 512 threads 189, 256 181, 128 179)
 constexpr int kRows = 4;       // of a thread (one 243 us, two 199, four 182, eight 183)
-constexpr int64_t kFewBlocks = 2048;  // of an SM: up to here a thread has one block
+// Blocks of an SM up to which a thread has one (us, one a thread / kRows, or two of ragged rows: bf16 rows of 1,024 with
+// dropout at 2,048 blocks an SM 8.2 / 9.7, at 4,096 12.3 / 10.3, at 8,192 16.5 / 14.3, without dropout 8.2 / 8.4, 10.3 / 10.3,
+// 14.4 / 13.1; fp16 rows of 1,001 to fp32 10.2 / 11.7, 14.4 / 14.5, 20.6 / 22.5).
+constexpr int64_t kFewBlocks = 2048;
 
 struct LookupArgs {
   const void* src;

@@ -9,7 +9,7 @@
 // them up, in the order of the pieces, so that the bits do not depend on who that is.
 //
 // What bounds it: for many wide rows HBM, at the 5 TB/s that rows read and written all over the place reach here (65,536 x
-// 1,024 fp16 to fp32 rows: 214 MB in 42 us behind a sort of 27); for fewer the chain sort, look-up of the entries, first rows,
+// 1,024 fp16 to fp32 rows: 214 MB in 40 us behind a sort of 27); for fewer the chain sort, look-up of the entries, first rows,
 // joins (8,192 x 2,048 bf16: 14 + 2 + 6 + 5 us).  With dropout the generator's 78 instructions a block come on top of some 50.
 #include "aside.cuh"
 #include "embedding_grad.cuh"
@@ -26,8 +26,12 @@ constexpr int kGroup = 16;     // pieces whose parts of a token are added up fir
 constexpr int kWindow = 256;   // sorted entries of a warp
 constexpr int kStages = 4;     // rows of a warp's ring (eight: as fast, and no room for the rows that sums are added to)
 constexpr int kSumWarps = 4;   // of a CTA
-// Warps of an SM that pieces are made for, so that all run at once (us, 65,536 x 1,024 fp16: 20 warps 66.7, 24 65.3, 28 74.4;
-// 8,192 x 2,048 bf16: 30.2, 30.2, 32.8; two micro-batches of 16,384 x 2,048: 120.3, 121.4, 122.5).
+// Warps of an SM that pieces are made for (us, 65,536 x 1,024 fp16: 20 warps 66.7, 24 65.3, 28 74.4; 8,192 x 2,048 bf16:
+// 30.2, 30.2, 32.8; two micro-batches of 16,384 x 2,048, a quarter of it padding: 120.3, 121.4, 122.5).  Pieces are a multiple
+// of 8 entries and counted over all positions, padding too, whose pieces are empty: of the 24 some 17 to 22 have work.  All
+// run at once but for sums that are added to fp32 rows: fp32 gradients then take 45 KB a CTA, of which five, not six, fit an
+// SM (without padding, 20 / 24 / 28 warps: fp32 16,384 x 2,048 99 / 118 / 100, 65,536 x 1,024 185 / 184 / 157, bf16 16,384 x
+// 2,048 added to fp32 59 / 73 / 60, to bf16 44.5 / 46 / 44).
 constexpr int kWarpsOfSm = 24;
 constexpr uint32_t kHead = 0x80000000u;
 
