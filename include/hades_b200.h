@@ -796,8 +796,8 @@ int hb_step_backward(hb_step_t* s, const hb_step_desc_t* d, const int64_t* ids, 
 /* the next; the values of a row are contiguous.  Pointers are aligned to what    */
 /* they point to, a workspace to 16 bytes.  The first call on a device            */
 /* allocates its status word: make it outside of a stream capture.  A gradient    */
-/* outside of captures makes a stream at its first call of a thread on a stream:  */
-/* zeros run there, beside the sort.                                              */
+/* outside of captures makes a stream at its first call of a thread on a stream   */
+/* (64 of them a thread): zeros run there, beside the sort.                       */
 /* ------------------------------------------------------------------------- */
 #define HB_TYPE_F32 0
 #define HB_TYPE_F16 1
